@@ -11,6 +11,9 @@ OUT = os.path.join(HERE, "libgeobpe.so")
 SOURCES = [os.path.join(CSRC, "geobpe.hip")]
 DEPS = SOURCES + [os.path.join(CSRC, "keyjson.h"), os.path.join(CSRC, "device.h"), os.path.join(CSRC, "kernels.h"), os.path.join(CSRC, "bin_dense.h"), os.path.join(CSRC, "merge.h"), os.path.join(CSRC, "featurize.h"), os.path.join(CSRC, "rmsd.h"), os.path.join(CSRC, "glue.h"), os.path.join(CSRC, "tail.h"), os.path.join(CSRC, "mid.h"), os.path.join(CSRC, "exchange.h"),
                   os.path.join(os.path.dirname(os.path.dirname(HERE)), "include", "geobpe.h")]
+# packed float32 instructions, which the compiler forms by itself, are kept out of every kernel (some of
+# their forms have given wrong results on this hardware); hipcc's host pass warns that it does not know the feature
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 ARCH = os.environ.get("GEOBPE_ARCH", "gfx950")
 
 
@@ -27,7 +30,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if all(os.path.getmtime(d) <= t for d in DEPS if os.path.exists(d)):
             return OUT
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-O3", "-fPIC", "-shared", "-std=c++17",
-           "-ffp-contract=off", "-Wall", "-Wno-unused-result", "-Wno-unused-value",
+           "-ffp-contract=off", *NO_PACKED_F32, "-Wall", "-Wno-unused-result", "-Wno-unused-value",
            "-Wno-unused-function", *SOURCES, "-o", OUT + ".tmp"]
     if verbose:
         print(" ".join(cmd))

@@ -11,7 +11,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 argv = sys.argv[1:]
 extra = argv[argv.index("--") + 1:] if "--" in argv else []
 flt = argv[0] if argv and argv[0] != "--" else ""
-cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "--cuda-device-only", "-c", "-o",
+cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "--cuda-device-only", "-c", "-o",
        "/dev/null", "-Rpass-analysis=kernel-resource-usage", *extra, os.path.join(ROOT, "pt-bpe_amd/csrc/geobpe.hip")]
 out = subprocess.run(cmd, capture_output=True, text=True).stderr
 rows, cur = {}, None
