@@ -347,6 +347,59 @@ int geobpe_run_exchange(geobpe_ctx *ctx, int64_t n_merges, int64_t *n_done);
 int geobpe_run_exchange_log(geobpe_ctx *ctx, int64_t n_merges, int64_t *n_done, int64_t *first, int64_t *h_out,
                             int64_t cap);
 
+/* ---- decoding: from a model's probabilities over this vocabulary's ids to ids that
+ * BPE.dequantize / recover take (the reference's sampler, bin/train.py:715-716, draws them one
+ * by one in torch; it has no drafts and no cache of its own) ----
+ * A drafted tree of nodes: node 0 is the last decided token (parents[0] = -1, else the whole
+ * sequence is absent), node i > 0 hangs on the present node parents[i] < i, else it is absent.
+ * At most 128 nodes.  Device pointers on `device`, ordered on `stream` (a hipStream_t; NULL: the
+ * default stream); nothing is allocated or waited for.  Strides are in elements (commit: bytes)
+ * and may be any multiple of 16 bytes where rows of a head are meant.  GEOBPE_EARG: sizes,
+ * alignment or a null pointer; the message is in geobpe_draft_error() (of this thread). */
+typedef struct {
+  const void *d_q, *d_k_cache, *d_v_cache, *d_k, *d_v; /* queries; pages; the nodes' own keys and values */
+  void *d_out;                                         /* seqs x nodes x heads x head_dim, contiguous */
+  const void *d_table, *d_lens, *d_parents;            /* int32 */
+  int64_t q_stride[3], k_stride[3], v_stride[3];       /* seq, node, head */
+  int64_t kc_stride[3], vc_stride[3];                  /* page, slot, head */
+  int64_t table_stride, parents_stride;                /* per sequence (parents: 0 = one tree for all) */
+  int64_t seqs, nodes, heads, kv_heads, head_dim, page_size, pages, max_pages, dtype; /* 0 bf16, 1 fp16 */
+  double scale;
+} geobpe_attend_args;
+/* out[b, i, h] = softmax(scale q k) v over the cache's first lens[b] positions (position x: page
+ * table[b, x / page_size], slot x % page_size) and the nodes on the path from the root to i, of
+ * kv head h / (heads / kv_heads).  Absent nodes: 0.  A length outside [0, max_pages page_size] or a
+ * page outside [0, pages) among those needed: the sequence's present rows are NaN. */
+int geobpe_tree_attention(int device, void *stream, const geobpe_attend_args *args);
+
+typedef struct {
+  const void *d_parents, *d_ids, *d_target, *d_draft; /* d_draft NULL: drafts without probabilities */
+  const void *d_u, *d_ranges, *d_start;               /* float32; int32 classes x 2; int32 per sequence */
+  void *d_n, *d_path, *d_tokens;                      /* int32: seqs; seqs x nodes; seqs x nodes */
+  int64_t target_stride[2], draft_stride[2];          /* seq, node; the vocabulary is contiguous */
+  int64_t parents_stride, ids_stride, u_stride;
+  int64_t seqs, nodes, vocab, classes, ids_int64, dtype; /* 0 bf16, 1 fp16, 2 fp32 */
+} geobpe_verify_args;
+/* Per sequence: node i's id is accepted when u[i] draft[parent, id] Z < r(id), r the target's row of
+ * the parent less what its rejected siblings took (r <- max(r - Z draft, 0), Z <- sum r, at first 1);
+ * the next id is the first whose cumulative r passes u[0] sum r.  n: the kept nodes, root
+ * included; path: their indices; tokens: the n - 1 accepted ids, then the next one; -1 behind. */
+int geobpe_verify_draft(int device, void *stream, const geobpe_verify_args *args);
+
+typedef struct {
+  const void *d_k, *d_v;                      /* layers x seqs x nodes x kv_heads x head_bytes */
+  void *d_k_cache, *d_v_cache;                /* layers x pages x page_size x kv_heads x head_bytes */
+  const void *d_table, *d_lens, *d_path, *d_n; /* int32 */
+  void *d_lens_out;                           /* int32; not d_lens itself */
+  int64_t k_stride[4], v_stride[4], kc_stride[4], vc_stride[4]; /* bytes: layer, seq | page, node | slot, head */
+  int64_t table_stride, path_stride;
+  int64_t layers, seqs, nodes, kv_heads, head_bytes, page_size, pages, max_pages;
+} geobpe_commit_args;
+/* cache[layer, position lens[b] + t] = node path[b, t] of sequence b for t < n[b]; lens_out = lens + n.
+ * A kept node outside the tree, the table or the pages is not written, and lens_out[b] is -1. */
+int geobpe_commit_draft(int device, void *stream, const geobpe_commit_args *args);
+const char *geobpe_draft_error(void);
+
 #ifdef __cplusplus
 }
 #endif

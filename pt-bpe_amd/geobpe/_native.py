@@ -132,6 +132,10 @@ def lib():
         "geobpe_run_exchange_log": (ctypes.c_int, [P, I64, pI64, pI64, P, I64]),
         "geobpe_comm_peer_active": (ctypes.c_int, [P]),
         "geobpe_collapsed": (ctypes.c_int, [P]),
+        "geobpe_tree_attention": (ctypes.c_int, [ctypes.c_int, P, P]),
+        "geobpe_verify_draft": (ctypes.c_int, [ctypes.c_int, P, P]),
+        "geobpe_commit_draft": (ctypes.c_int, [ctypes.c_int, P, P]),
+        "geobpe_draft_error": (ctypes.c_char_p, []),
     }
     ab = bool(os.environ.get("GEOBPE_LIB"))  # (an older A/B build may lack this round's entry points)
     for name, (res, args) in sig.items():
@@ -159,7 +163,8 @@ EXPORTED_SYMBOLS = [
     "geobpe_comm_set_slot", "geobpe_run_exchange", "geobpe_pdb_backbone", "geobpe_pdb_error",
     "geobpe_featurize", "geobpe_rmsd", "geobpe_nerf", "geobpe_glue_opt", "geobpe_arena_release",
     "geobpe_set_collapse", "geobpe_collapsed", "geobpe_comm_peer", "geobpe_comm_peer_active",
-    "geobpe_run_exchange_log",
+    "geobpe_run_exchange_log", "geobpe_tree_attention", "geobpe_verify_draft", "geobpe_commit_draft",
+    "geobpe_draft_error",
 ]
 
 

@@ -13,6 +13,7 @@ mode uses, so a caller of the reference (bin/encode.py, train.py) can switch:
   bpe.dequantize / recover               same                         bpe.py:959-1002
   bpe.vocab_size / cum_bin_count(key)    same                         bpe.py:878-915
   bpe.capacity(tokenizer=False)          same                         bpe.py:885-902
+  (sampling in train.py, id by id)       bpe.verify_draft(...)        drafted ids on the device (geobpe.draft)
   bpe._tokens / _thresholds / _step      same contents
   bpe.tokenizers[i].bond_to_token, .token_pos, .tokens, .tokenize(), .n
 
@@ -492,6 +493,36 @@ class BPE:
         bond_to_token, token_geo, tokenize, compute_coords) built from recovered geometry."""
         from .rmsd_bpe import recover_structure
         return recover_structure(self._tokens, repl, tokenized, self._engine.device)
+
+    def id_ranges(self, device=None):
+        """The ids [lo, hi) that can stand at each place of an encoded chain, by place % 4: a motif, then the
+        junction's omega, phi and C:1N:1CA (tokenizer.py:379-392, bpe.py:946-954).  (4, 2) int32: numpy, or with
+        ``device`` a torch tensor there, made once per vocabulary (before a graph capture that needs it)."""
+        if not self.res_init:
+            raise NotImplementedError("bond-level init has no fixed order of motifs and junction angles")
+        K = len(self._tokens)
+        lo = [0] + [K + self.cum_bin_count(k) for k in GLUE_KEYS]
+        r = np.array([[a, a + (self.B if i else K)] for i, a in enumerate(lo)], dtype=np.int32)
+        if device is None:
+            return r
+        import torch
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        kept = getattr(self, "_id_ranges", None)
+        if kept is None or kept[0] != (K, device):
+            kept = self._id_ranges = ((K, device), torch.tensor(r, device=device))
+        return kept[1]
+
+    def verify_draft(self, parents, ids, target, draft, u, start):
+        """Drafted ids against a model's probabilities over this vocabulary (geobpe.draft.verify), each place
+        held to its kind of id (``id_ranges``): start[b] is the place in the chain of the token after the root,
+        i.e. the number of ids decided so far.  A row may be wider than vocab_size (a model's own extra ids lie
+        behind it); those are never drawn here.  ``tokens`` of the result is what dequantize / recover take."""
+        from . import draft as _draft
+        if target.shape[-1] < self.vocab_size:
+            raise ValueError(f"rows of {target.shape[-1]} probabilities for {self.vocab_size} ids")
+        return _draft.verify(parents, ids, target, draft, u, ranges=self.id_ranges(target.device), start=start)
 
     def capacity(self, tokenizer=False):
         """bpe.py:885-902."""

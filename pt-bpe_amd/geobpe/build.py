@@ -8,8 +8,9 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "csrc")
 OUT = os.path.join(HERE, "libgeobpe.so")
-SOURCES = [os.path.join(CSRC, "geobpe.hip")]
+SOURCES = [os.path.join(CSRC, "geobpe.hip"), os.path.join(CSRC, "draft.hip")]
 DEPS = SOURCES + [os.path.join(CSRC, "keyjson.h"), os.path.join(CSRC, "device.h"), os.path.join(CSRC, "kernels.h"), os.path.join(CSRC, "bin_dense.h"), os.path.join(CSRC, "merge.h"), os.path.join(CSRC, "featurize.h"), os.path.join(CSRC, "rmsd.h"), os.path.join(CSRC, "glue.h"), os.path.join(CSRC, "tail.h"), os.path.join(CSRC, "mid.h"), os.path.join(CSRC, "exchange.h"),
+                  *(os.path.join(CSRC, h) for h in ("draft.h", "draft_attend.h", "draft_verify.h", "draft_commit.h")),
                   os.path.join(os.path.dirname(os.path.dirname(HERE)), "include", "geobpe.h")]
 # packed float32 instructions, which the compiler forms by itself, are kept out of every kernel (some of
 # their forms have given wrong results on this hardware); hipcc's host pass warns that it does not know the feature

@@ -1309,6 +1309,14 @@ class RmsdBPE:
         from .bpe import BPE
         return BPE.recover(self, tokenized)
 
+    def id_ranges(self, device=None):
+        from .bpe import BPE
+        return BPE.id_ranges(self, device)
+
+    def verify_draft(self, parents, ids, target, draft, u, start):
+        from .bpe import BPE
+        return BPE.verify_draft(self, parents, ids, target, draft, u, start)
+
     def encode_all(self):
         """quantize(tokenize()) of every chain as (ids, row offsets)."""
         q = [self.quantize(t) for t in self.tokenizers]

@@ -3,5 +3,5 @@
 set -e
 cd "$(dirname "$0")/.."
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -fPIC -shared -std=c++17 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops -Wall -Wno-unused-result \
-  -Wno-unused-value -Wno-unused-function $2 pt-bpe_amd/csrc/geobpe.hip -o pt-bpe_amd/geobpe/ab_$1.so
+  -Wno-unused-value -Wno-unused-function $2 pt-bpe_amd/csrc/geobpe.hip pt-bpe_amd/csrc/draft.hip -o pt-bpe_amd/geobpe/ab_$1.so
 echo pt-bpe_amd/geobpe/ab_$1.so
