@@ -370,7 +370,9 @@ typedef struct {
  * table[b, x / page_size], slot x % page_size) and the nodes on the path from the root to i, of
  * kv head h / (heads / kv_heads).  Absent nodes: 0.  A length outside [0, max_pages page_size] or a
  * page outside [0, pages) among those needed: the sequence's present rows are NaN. */
-int geobpe_tree_attention(int device, void *stream, const geobpe_attend_args *args);
+int geobpe_tree_attention(int device, void *stream, const geobpe_attend_args *args, void *d_work, int64_t work_bytes);
+/* bytes of d_work (16-byte aligned, this call's alone until it is done; 0: none), -1: sizes out of range */
+int64_t geobpe_tree_attention_work(const geobpe_attend_args *args);
 
 typedef struct {
   const void *d_parents, *d_ids, *d_target, *d_draft; /* d_draft NULL: drafts without probabilities */

@@ -11,6 +11,7 @@
 namespace gb {
 
 constexpr int DRAFT_MAX_NODES = 128;
+constexpr int DRAFT_MAX_POSITIONS = 0x7fffffc0;  // a sequence's; a tile of keys more stays an int32
 
 // depth of node i (root: 0), -1 when it is absent.  par: the tree's parents (N of them, LDS).
 // Every step goes to a smaller index, so the walk ends within i steps.
@@ -25,43 +26,40 @@ __device__ inline int draft_depth(const int* par, int i) {
   return par[0] == -1 ? d : -1;
 }
 
-// x / d for 0 <= x < 2^31 and 1 <= d < 2^31, with the host's m = floor(2^32 / d) + 1: x m / 2^32 is
-// at least x / d and above it by less than x / 2^32 < 1/2, so its floor is the quotient or one more,
-// which the remainder's sign tells.
+// x / d for 0 <= x < 2^31 and 1 <= d < 2^31, with the host's m = min(2^32 / d, 2^32 - 1) rounded down: x m / 2^32
+// is at most x / d and below it by less than x / 2^32 < 1/2, so its floor is the quotient or one less, which the
+// remainder tells.
 struct PageDiv {
   uint32_t m;
   int32_t d;
 };
-inline PageDiv page_div(int32_t d) { return {d == 1 ? 0u : (uint32_t)((1ull << 32) / (uint32_t)d + 1), d}; }
+inline PageDiv page_div(int32_t d) { return {d == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)d), d}; }
 __device__ inline void page_split(PageDiv v, int x, int& page, int& slot) {
-  if (v.d == 1) {
-    page = x;
-    slot = 0;
-    return;
-  }
-  int q = (int)__umulhi((uint32_t)x, v.m);
-  int r = (int)((uint32_t)x - (uint32_t)q * (uint32_t)v.d);
-  if (r < 0) {
-    q--;
-    r += v.d;
-  }
-  page = q;
-  slot = r;
+  const uint32_t q = __umulhi((uint32_t)x, v.m), r = (uint32_t)x - q * (uint32_t)v.d;
+  const bool more = r >= (uint32_t)v.d;
+  page = (int)(q + more);
+  slot = (int)(more ? r - v.d : r);
 }
 
-// where position x of a sequence lies: slot and page, the page -1 where the table's entry is none of
-// the cache's P pages or x is past the table's M entries.  Nothing is read outside the table.
+// A sequence's row of the table: position x lies in slot x % S of page row[x / S].
 struct Pages {
-  const int32_t* row;  // the sequence's entries
+  const int32_t* row;  // M entries
   PageDiv div;
   int32_t P, M;
 };
-__device__ inline int find_page(const Pages& t, int x, int& slot) {
+// the table's entry for 0 <= x < M S, as it is: good_page has to pass it before it is used
+__device__ inline int page_entry(const Pages& t, int x, int& slot) {
   int k;
   page_split(t.div, x, k, slot);
-  if (x < 0 || k >= t.M) return -1;
-  const int id = t.row[k];
-  return id >= 0 && id < t.P ? id : -1;
+  return t.row[k];
+}
+__device__ inline bool good_page(const Pages& t, int id) { return (uint32_t)id < (uint32_t)t.P; }
+// for any x: the page, or -1 where the entry is none of the cache's P pages or x is not in the table (which
+// is not read then)
+__device__ inline int find_page(const Pages& t, int x, int& slot) {
+  if (x < 0 || x / t.div.d >= t.M) return -1;
+  const int id = page_entry(t, x, slot);
+  return good_page(t, id) ? id : -1;
 }
 
 }  // namespace gb

@@ -4,6 +4,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "../../include/geobpe.h"
 #include "draft_attend.h"
 #include "draft_commit.h"
@@ -46,27 +48,100 @@ bool aligned(const void* p, const int64_t* strides, int n, int64_t unit) {
     if (strides[i] % unit) return false;
   return true;
 }
+
+// how a call is cut: rows a workgroup works on, parts of the keys
+struct AttendPlan {
+  bool wide;
+  int rb, rows, tile, splits;
+  int64_t row_tiles, blocks, bytes;
+};
+AttendPlan attend_plan(const geobpe_attend_args& x) {
+  AttendPlan p;
+  const int64_t M = x.nodes * (x.heads / x.kv_heads);
+  p.wide = M > 32;
+  p.rb = M <= 16 ? 1 : 2;
+  p.rows = p.wide ? WIDE_ROWS : 16 * p.rb;
+  p.tile = p.wide ? WIDE_TILE : ATT_TILE;
+  p.row_tiles = (M + p.rows - 1) / p.rows;
+  const int64_t tiles = (x.max_pages * x.page_size + p.tile - 1) / p.tile + (x.nodes + p.tile - 1) / p.tile;
+  const int64_t items = x.seqs * x.kv_heads, most = parts_of((int)tiles, INT32_MAX);
+  const int64_t want = ATT_WANT / (items * p.row_tiles);
+  p.splits = (int)(want < 1 ? 1 : want < most ? want : most);
+  p.blocks = (items * p.splits + 7) / 8 * 8 * p.row_tiles;
+  p.bytes = p.splits > 1 ? items * p.row_tiles * p.splits * p.rows * (x.head_dim + 2) * 4 : 0;
+  return p;
+}
+int attend_sizes(const geobpe_attend_args& x) {
+  if (x.seqs < 0 || x.nodes < 1 || x.nodes > DRAFT_MAX_NODES || x.kv_heads < 1 || x.heads < x.kv_heads ||
+      x.heads % x.kv_heads || x.head_dim < 8 || x.head_dim > 256 || x.head_dim % 8 || x.page_size < 1 || x.pages < 1 ||
+      x.max_pages < 0 || x.dtype < 0 || x.dtype > 1 || x.seqs > 65535 || x.heads > 65535 || x.pages > INT32_MAX ||
+      x.page_size > DRAFT_MAX_POSITIONS || x.max_pages > DRAFT_MAX_POSITIONS / x.page_size)
+    return fail(GEOBPE_EARG, "tree attention: sizes out of range");
+  if (x.seqs && attend_plan(x).blocks > INT32_MAX / ATT_BLOCK)
+    return fail(GEOBPE_EARG, "tree attention: %lld sequences of %lld rows are too many for one call", (long long)x.seqs,
+                (long long)(x.nodes * x.heads));
+  return GEOBPE_OK;
+}
+
+template <typename T, int KS>
+void attend_narrow(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
+  const dim3 grid((unsigned)p.blocks), block(ATT_BLOCK);
+  if (p.rb == 1)
+    hipLaunchKernelGGL((k_attend<T, KS, 1>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((k_attend<T, KS, 2>), grid, block, 0, s, a);
+}
+template <typename T>
+void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
+  const dim3 grid((unsigned)p.blocks), block(ATT_BLOCK);
+  if (p.wide) {
+    if (a.D <= 64)
+      hipLaunchKernelGGL((k_attend_wide<T, 64>), grid, block, 0, s, a);
+    else if (a.D <= 128)
+      hipLaunchKernelGGL((k_attend_wide<T, 128>), grid, block, 0, s, a);
+    else
+      hipLaunchKernelGGL((k_attend_wide<T, 256>), grid, block, 0, s, a);
+  } else {
+    switch ((a.D + 31) / 32) {
+      case 1: attend_narrow<T, 1>(a, p, s); break;
+      case 2: attend_narrow<T, 2>(a, p, s); break;
+      case 3: attend_narrow<T, 3>(a, p, s); break;
+      case 4: attend_narrow<T, 4>(a, p, s); break;
+      default: attend_narrow<T, 8>(a, p, s);
+    }
+  }
+  if (p.splits > 1) {
+    const int64_t rows = (int64_t)a.B * a.N * a.Hq;
+    hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)((rows + ATT_WAVES - 1) / ATT_WAVES)), dim3(ATT_BLOCK), 0, s, a,
+                       p.rows, p.tile);
+  }
+}
 }  // namespace
 
 extern "C" {
 
 const char* geobpe_draft_error(void) { return g_draft_error; }
 
-int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p) {
+int64_t geobpe_tree_attention_work(const geobpe_attend_args* p) {
+  if (!p || attend_sizes(*p) != GEOBPE_OK) return -1;
+  return p->seqs ? attend_plan(*p).bytes : 0;
+}
+
+int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p, void* d_work, int64_t work_bytes) {
   if (!p) return fail(GEOBPE_EARG, "no arguments");
   const geobpe_attend_args& x = *p;
-  if (x.seqs < 0 || x.nodes < 1 || x.nodes > DRAFT_MAX_NODES || x.kv_heads < 1 || x.heads < x.kv_heads ||
-      x.heads % x.kv_heads || x.head_dim < 8 || x.head_dim > 256 || x.head_dim % 8 || x.page_size < 1 || x.pages < 1 ||
-      x.max_pages < 0 || x.dtype < 0 || x.dtype > 1 || x.seqs > 65535 || x.heads > 65535 || x.pages > INT32_MAX ||
-      x.page_size > INT32_MAX || x.max_pages > INT32_MAX / x.page_size)
-    return fail(GEOBPE_EARG, "tree attention: sizes out of range");
-  if (x.seqs == 0) return GEOBPE_OK;
+  const int rc = attend_sizes(x);
+  if (rc != GEOBPE_OK || x.seqs == 0) return rc;
+  const AttendPlan plan = attend_plan(x);
   if (!x.d_q || !x.d_k_cache || !x.d_v_cache || !x.d_k || !x.d_v || !x.d_lens || !x.d_parents || !x.d_out ||
-      (x.max_pages && !x.d_table))
+      (x.max_pages && !x.d_table) || (plan.bytes && !d_work))
     return fail(GEOBPE_EARG, "tree attention: null pointer");
+  if (work_bytes < plan.bytes)
+    return fail(GEOBPE_EARG, "tree attention: %lld bytes of work space, %lld are needed", (long long)work_bytes,
+                (long long)plan.bytes);
   if (!aligned(x.d_q, x.q_stride, 3, 8) || !aligned(x.d_k_cache, x.kc_stride, 3, 8) ||
       !aligned(x.d_v_cache, x.vc_stride, 3, 8) || !aligned(x.d_k, x.k_stride, 3, 8) ||
-      !aligned(x.d_v, x.v_stride, 3, 8) || (uintptr_t)x.d_out % 16)
+      !aligned(x.d_v, x.v_stride, 3, 8) || (uintptr_t)x.d_out % 16 || (uintptr_t)d_work % 16)
     return fail(GEOBPE_EARG, "tree attention: rows are not 16-byte aligned");
   AttendArgs a;
   a.q = x.d_q, a.kc = x.d_k_cache, a.vc = x.d_v_cache, a.kd = x.d_k, a.vd = x.d_v, a.out = x.d_out;
@@ -80,13 +155,14 @@ int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p)
   a.S = (int)x.page_size, a.P = (int)x.pages, a.M = (int)x.max_pages;
   a.div = page_div(a.S);
   a.scale = (float)x.scale;
+  a.splits = plan.splits;
+  a.part = (float*)d_work;
   OnDevice on(device);
   if (!on.ok) return fail(GEOBPE_EHIP, "tree attention: device %d", device);
-  const dim3 grid((unsigned)(a.N * a.Hq), (unsigned)a.B);
   if (x.dtype == 0)
-    hipLaunchKernelGGL(k_attend_row<bf16_t>, grid, dim3(ATT_BLOCK), 0, (hipStream_t)stream, a);
+    attend_launch<bf16_t>(a, plan, (hipStream_t)stream);
   else
-    hipLaunchKernelGGL(k_attend_row<fp16_t>, grid, dim3(ATT_BLOCK), 0, (hipStream_t)stream, a);
+    attend_launch<fp16_t>(a, plan, (hipStream_t)stream);
   return launched("tree attention");
 }
 
@@ -133,8 +209,8 @@ int geobpe_commit_draft(int device, void* stream, const geobpe_commit_args* p) {
   const geobpe_commit_args& x = *p;
   if (x.layers < 1 || x.layers > 65535 || x.seqs < 0 || x.nodes < 1 || x.nodes > DRAFT_MAX_NODES || x.kv_heads < 1 ||
       x.kv_heads > 65535 || x.head_bytes < 16 || x.head_bytes > 65536 || x.head_bytes % 16 || x.page_size < 1 ||
-      x.pages < 1 || x.max_pages < 0 || x.pages > INT32_MAX || x.page_size > INT32_MAX ||
-      x.max_pages > INT32_MAX / x.page_size || x.seqs > INT32_MAX / x.nodes)
+      x.pages < 1 || x.max_pages < 0 || x.pages > INT32_MAX || x.page_size > DRAFT_MAX_POSITIONS ||
+      x.max_pages > DRAFT_MAX_POSITIONS / x.page_size || x.seqs > INT32_MAX / x.nodes)
     return fail(GEOBPE_EARG, "commit: sizes out of range");
   if (x.seqs == 0) return GEOBPE_OK;
   if (!x.d_k || !x.d_v || !x.d_k_cache || !x.d_v_cache || !x.d_lens || !x.d_path || !x.d_n || !x.d_lens_out ||
@@ -155,7 +231,7 @@ int geobpe_commit_draft(int device, void* stream, const geobpe_commit_args* p) {
   a.div = page_div(a.S);
   OnDevice on(device);
   if (!on.ok) return fail(GEOBPE_EHIP, "commit: device %d", device);
-  hipLaunchKernelGGL(k_commit, dim3((unsigned)(a.B * a.N), (unsigned)a.L), dim3(256), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(k_commit_nodes, dim3((unsigned)(a.B * a.N), (unsigned)a.L), dim3(256), 0, (hipStream_t)stream, a);
   return launched("commit");
 }
 

@@ -25,7 +25,7 @@ struct alignas(16) Piece {
 };
 
 // One workgroup per kept node and layer.
-__global__ __launch_bounds__(256) void k_commit(CommitArgs a) {
+__global__ __launch_bounds__(256) void k_commit_nodes(CommitArgs a) {
   const int t = blockIdx.x % a.N, b = blockIdx.x / a.N, layer = blockIdx.y;
   const int len = a.lens[b], n = min(a.n[b], a.N);
   // a sequence with a node outside the tree or the cache is left as it is in that node, its length -1

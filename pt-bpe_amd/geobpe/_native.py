@@ -132,7 +132,8 @@ def lib():
         "geobpe_run_exchange_log": (ctypes.c_int, [P, I64, pI64, pI64, P, I64]),
         "geobpe_comm_peer_active": (ctypes.c_int, [P]),
         "geobpe_collapsed": (ctypes.c_int, [P]),
-        "geobpe_tree_attention": (ctypes.c_int, [ctypes.c_int, P, P]),
+        "geobpe_tree_attention": (ctypes.c_int, [ctypes.c_int, P, P, P, I64]),
+        "geobpe_tree_attention_work": (I64, [P]),
         "geobpe_verify_draft": (ctypes.c_int, [ctypes.c_int, P, P]),
         "geobpe_commit_draft": (ctypes.c_int, [ctypes.c_int, P, P]),
         "geobpe_draft_error": (ctypes.c_char_p, []),
@@ -163,7 +164,7 @@ EXPORTED_SYMBOLS = [
     "geobpe_comm_set_slot", "geobpe_run_exchange", "geobpe_pdb_backbone", "geobpe_pdb_error",
     "geobpe_featurize", "geobpe_rmsd", "geobpe_nerf", "geobpe_glue_opt", "geobpe_arena_release",
     "geobpe_set_collapse", "geobpe_collapsed", "geobpe_comm_peer", "geobpe_comm_peer_active",
-    "geobpe_run_exchange_log", "geobpe_tree_attention", "geobpe_verify_draft", "geobpe_commit_draft",
+    "geobpe_run_exchange_log", "geobpe_tree_attention", "geobpe_tree_attention_work", "geobpe_verify_draft", "geobpe_commit_draft",
     "geobpe_draft_error",
 ]
 

@@ -26,7 +26,7 @@ from . import _native
 
 MAX_NODES = 128
 MAX_VOCAB = 1 << 22
-MAX_POSITIONS = (1 << 31) - 1
+MAX_POSITIONS = (1 << 31) - 64
 
 _HALF = {torch.bfloat16: 0, torch.float16: 1}
 _PROB = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -158,7 +158,10 @@ def tree_attention(q, k_cache, v_cache, block_table, lens, k, v, parents, scale:
         block_table.data_ptr(), lens.data_ptr(), parents.data_ptr(), *rows, block_table.stride(0), ps,
         B, N, Hq, Hkv, D, S, P, M,
         _HALF[q.dtype], D ** -0.5 if scale is None else float(scale))
-    _call(_native.lib().geobpe_tree_attention(dev.index, stream, args))
+    lib = _native.lib()
+    need = lib.geobpe_tree_attention_work(args)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _call(lib.geobpe_tree_attention(dev.index, stream, args, work.data_ptr() if need > 0 else None, need))
     return out
 
 

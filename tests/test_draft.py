@@ -329,22 +329,30 @@ def test_c_entries_refuse_without_a_device():
     """The C entries check sizes, pointers and alignment before they touch a device."""
     from geobpe import _native
     L = _native.lib()
-    assert L.geobpe_tree_attention(0, None, None) == _native.E_ARG
+    assert L.geobpe_tree_attention(0, None, None, None, 0) == _native.E_ARG
     ok = dict(ptr=[256] * 9, st=[64, 64, 64] * 5, rest=[1, 0], sizes=[1, 2, 4, 2, 64, 16, 3, 2, 0])
     pack = lambda d: draft._ATTEND.pack(*d["ptr"], *d["st"], *d["rest"], *d["sizes"], 1.0)  # noqa: E731
     for i, bad in ((0, -1), (1, 0), (1, 129), (2, 3), (3, 0), (4, 60), (4, 264), (5, 0), (6, 0), (7, 1 << 31), (8, 2)):
         d = {**ok, "sizes": [bad if j == i else x for j, x in enumerate(ok["sizes"])]}
-        assert L.geobpe_tree_attention(0, None, pack(d)) == _native.E_ARG, (i, bad)
+        assert L.geobpe_tree_attention(0, None, pack(d), 256, 1 << 40) == _native.E_ARG, (i, bad)
         assert b"sizes" in L.geobpe_draft_error()
+        assert L.geobpe_tree_attention_work(pack(d)) == -1
+    long = {**ok, "sizes": [1, 2, 4, 2, 64, 16, 3, 1000, 0]}
+    need = L.geobpe_tree_attention_work(pack(long))
+    assert need > 0 and L.geobpe_tree_attention_work(pack({**ok, "sizes": [0, *ok["sizes"][1:]]})) == 0
+    assert L.geobpe_tree_attention(0, None, pack(long), 256, need - 1) == _native.E_ARG
+    assert b"work space" in L.geobpe_draft_error()
+    assert L.geobpe_tree_attention(0, None, pack(long), None, need) == _native.E_ARG
+    assert L.geobpe_tree_attention(0, None, pack(long), 264, need) == _native.E_ARG
     for i in range(9):
         d = {**ok, "ptr": [0 if j == i else x for j, x in enumerate(ok["ptr"])]}
-        assert L.geobpe_tree_attention(0, None, pack(d)) == _native.E_ARG and b"null" in L.geobpe_draft_error()
+        assert L.geobpe_tree_attention(0, None, pack(d), 256, 1 << 40) == _native.E_ARG and b"null" in L.geobpe_draft_error()
     d = {**ok, "ptr": [256 + 2, *ok["ptr"][1:]]}
-    assert L.geobpe_tree_attention(0, None, pack(d)) == _native.E_ARG and b"aligned" in L.geobpe_draft_error()
+    assert L.geobpe_tree_attention(0, None, pack(d), 256, 1 << 40) == _native.E_ARG and b"aligned" in L.geobpe_draft_error()
     d = {**ok, "st": [65, *ok["st"][1:]]}
-    assert L.geobpe_tree_attention(0, None, pack(d)) == _native.E_ARG and b"aligned" in L.geobpe_draft_error()
+    assert L.geobpe_tree_attention(0, None, pack(d), 256, 1 << 40) == _native.E_ARG and b"aligned" in L.geobpe_draft_error()
     d = {**ok, "sizes": [0, *ok["sizes"][1:]]}
-    assert L.geobpe_tree_attention(0, None, pack(d)) == 0  # no sequences: nothing to do
+    assert L.geobpe_tree_attention(0, None, pack(d), 256, 1 << 40) == 0  # no sequences: nothing to do
     assert L.geobpe_verify_draft(0, None, None) == _native.E_ARG
     v = [256] * 10 + [8, 8, 8, 8, 0, 4, 4]
     for i, bad in ((0, -1), (1, 0), (1, 129), (2, 0), (2, (1 << 22) + 1), (3, -1), (5, 3)):
