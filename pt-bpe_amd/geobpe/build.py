@@ -68,6 +68,35 @@ def build_keys(force: bool = False, verbose: bool = False) -> str:
     return KEY_OUT
 
 
+DRAFT_SRC = os.path.join(CSRC, "draft_py.cpp")
+DRAFT_OUT = os.path.join(HERE, "_draft.so")
+
+
+def build_draft(force: bool = False, verbose: bool = False) -> str:
+    """The decoding operators' Python side (csrc/draft_py.cpp), a CPython extension over the installed PyTorch."""
+    import sysconfig
+    header = os.path.join(os.path.dirname(os.path.dirname(HERE)), "include", "geobpe.h")
+    if not force and os.path.exists(DRAFT_OUT) and all(os.path.getmtime(f) <= os.path.getmtime(DRAFT_OUT)
+                                                       for f in (DRAFT_SRC, header)):
+        return DRAFT_OUT
+    import torch
+    from torch.utils import cpp_extension
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-shared", "-fPIC", "-std=c++17", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+           "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-I{sysconfig.get_paths()['include']}",
+           *(f"-isystem{d}" for d in cpp_extension.include_paths("cuda")), DRAFT_SRC, f"-L{lib}",
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip", "-o", DRAFT_OUT + ".tmp"]
+    if verbose:
+        print(" ".join(cmd))
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed:\n{r.stderr[-4000:]}")
+    os.replace(DRAFT_OUT + ".tmp", DRAFT_OUT)
+    return DRAFT_OUT
+
+
 if __name__ == "__main__":
     print(build(force=True, verbose=True))
     print(build_keys(force=True, verbose=True))
+    print(build_draft(force=True, verbose=True))
