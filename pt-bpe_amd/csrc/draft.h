@@ -11,7 +11,7 @@
 namespace gb {
 
 constexpr int DRAFT_MAX_NODES = 128;
-constexpr int DRAFT_MAX_POSITIONS = 0x7fffffc0;  // a sequence's; a tile of keys more stays an int32
+constexpr int DRAFT_MAX_POSITIONS = 0x7ffff000;  // a sequence's; some tiles of keys more stay an int32
 
 // depth of node i (root: 0), -1 when it is absent.  par: the tree's parents (N of them, LDS).
 // Every step goes to a smaller index, so the walk ends within i steps.

@@ -49,10 +49,10 @@ bool aligned(const void* p, const int64_t* strides, int n, int64_t unit) {
   return true;
 }
 
-// how a call is cut: rows a workgroup works on, parts of the keys
+// how a call is cut: rows a workgroup works on, tiles of keys a part has at most
 struct AttendPlan {
   bool wide;
-  int rb, rows, tile, splits;
+  int rb, rows, tile, per, most;
   int64_t row_tiles, blocks, bytes;
 };
 AttendPlan attend_plan(const geobpe_attend_args& x) {
@@ -64,11 +64,11 @@ AttendPlan attend_plan(const geobpe_attend_args& x) {
   p.tile = p.wide ? WIDE_TILE : ATT_TILE;
   p.row_tiles = (M + p.rows - 1) / p.rows;
   const int64_t tiles = (x.max_pages * x.page_size + p.tile - 1) / p.tile + (x.nodes + p.tile - 1) / p.tile;
-  const int64_t items = x.seqs * x.kv_heads, most = parts_of((int)tiles, INT32_MAX);
-  const int64_t want = ATT_WANT / (items * p.row_tiles);
-  p.splits = (int)(want < 1 ? 1 : want < most ? want : most);
-  p.blocks = (items * p.splits + 7) / 8 * 8 * p.row_tiles;
-  p.bytes = p.splits > 1 ? items * p.row_tiles * p.splits * p.rows * (x.head_dim + 2) * 4 : 0;
+  const int64_t items = x.seqs * x.kv_heads, even = (items * p.row_tiles * tiles + ATT_WANT - 1) / ATT_WANT;
+  p.per = (int)(even > tiles ? tiles : even > ATT_LEAST ? even : ATT_LEAST);
+  p.most = (int)((tiles + p.per - 1) / p.per);
+  p.blocks = (items * p.most + 7) / 8 * 8 * p.row_tiles;
+  p.bytes = p.most > 1 ? items * p.row_tiles * p.most * p.rows * (x.head_dim + 2) * 4 : 0;
   return p;
 }
 int attend_sizes(const geobpe_attend_args& x) {
@@ -77,7 +77,9 @@ int attend_sizes(const geobpe_attend_args& x) {
       x.max_pages < 0 || x.dtype < 0 || x.dtype > 1 || x.seqs > 65535 || x.heads > 65535 || x.pages > INT32_MAX ||
       x.page_size > DRAFT_MAX_POSITIONS || x.max_pages > DRAFT_MAX_POSITIONS / x.page_size)
     return fail(GEOBPE_EARG, "tree attention: sizes out of range");
-  if (x.seqs && attend_plan(x).blocks > INT32_MAX / ATT_BLOCK)
+  if (x.seqs == 0) return GEOBPE_OK;
+  if (x.seqs * x.nodes * x.heads > INT32_MAX / ATT_BLOCK ||
+      attend_plan(x).blocks > INT32_MAX / ATT_BLOCK)
     return fail(GEOBPE_EARG, "tree attention: %lld sequences of %lld rows are too many for one call", (long long)x.seqs,
                 (long long)(x.nodes * x.heads));
   return GEOBPE_OK;
@@ -110,10 +112,15 @@ void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
       default: attend_narrow<T, 8>(a, p, s);
     }
   }
-  if (p.splits > 1) {
+  if (p.most > 1) {
+    // eight threads over a row's parts where there are too few rows to fill the card
     const int64_t rows = (int64_t)a.B * a.N * a.Hq;
-    hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)((rows + ATT_WAVES - 1) / ATT_WAVES)), dim3(ATT_BLOCK), 0, s, a,
-                       p.rows, p.tile);
+    const int by = rows * (a.D / 4) < 512 * ATT_BLOCK && a.D <= 128 ? 8 : 1, each = ATT_BLOCK / (a.D / 4 * by);
+    const dim3 joins((unsigned)((rows + each - 1) / each));
+    if (by == 8)
+      hipLaunchKernelGGL((k_attend_join<T, 8>), joins, block, 0, s, a, p.rows, p.tile);
+    else
+      hipLaunchKernelGGL((k_attend_join<T, 1>), joins, block, 0, s, a, p.rows, p.tile);
   }
 }
 }  // namespace
@@ -143,19 +150,23 @@ int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p,
       !aligned(x.d_v_cache, x.vc_stride, 3, 8) || !aligned(x.d_k, x.k_stride, 3, 8) ||
       !aligned(x.d_v, x.v_stride, 3, 8) || (uintptr_t)x.d_out % 16 || (uintptr_t)d_work % 16)
     return fail(GEOBPE_EARG, "tree attention: rows are not 16-byte aligned");
+  for (int i = 0; i < 2; i++)
+    if (x.kc_stride[i] < 0 || x.vc_stride[i] < 0 || x.kc_stride[i] / 8 > UINT32_MAX || x.vc_stride[i] / 8 > UINT32_MAX)
+      return fail(GEOBPE_EARG, "tree attention: a page or slot of the cache spans more than 64 GiB");
   AttendArgs a;
   a.q = x.d_q, a.kc = x.d_k_cache, a.vc = x.d_v_cache, a.kd = x.d_k, a.vd = x.d_v, a.out = x.d_out;
   a.table = (const int32_t*)x.d_table, a.lens = (const int32_t*)x.d_lens, a.parents = (const int32_t*)x.d_parents;
-  for (int i = 0; i < 3; i++) {
-    a.qs[i] = x.q_stride[i], a.kcs[i] = x.kc_stride[i], a.vcs[i] = x.vc_stride[i];
-    a.kds[i] = x.k_stride[i], a.vds[i] = x.v_stride[i];
-  }
+  for (int i = 0; i < 3; i++) a.qs[i] = x.q_stride[i], a.kds[i] = x.k_stride[i], a.vds[i] = x.v_stride[i];
+  a.khead = x.kc_stride[2], a.vhead = x.vc_stride[2];
+  a.kpage = (uint32_t)(x.kc_stride[0] / 8), a.kslot = (uint32_t)(x.kc_stride[1] / 8);
+  a.vpage = (uint32_t)(x.vc_stride[0] / 8), a.vslot = (uint32_t)(x.vc_stride[1] / 8);
   a.table_stride = x.table_stride, a.parents_stride = x.parents_stride;
   a.B = (int)x.seqs, a.N = (int)x.nodes, a.Hq = (int)x.heads, a.Hkv = (int)x.kv_heads, a.D = (int)x.head_dim;
   a.S = (int)x.page_size, a.P = (int)x.pages, a.M = (int)x.max_pages;
   a.div = page_div(a.S);
   a.scale = (float)x.scale;
-  a.splits = plan.splits;
+  a.per = plan.per;
+  a.most = plan.most;
   a.part = (float*)d_work;
   OnDevice on(device);
   if (!on.ok) return fail(GEOBPE_EHIP, "tree attention: device %d", device);

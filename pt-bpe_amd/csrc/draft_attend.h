@@ -17,29 +17,34 @@ struct AttendArgs {
   const void *q, *kc, *vc, *kd, *vd;
   void* out;
   const int32_t *table, *lens, *parents;
-  int64_t qs[3], kcs[3], vcs[3], kds[3], vds[3];  // strides: (seq, node, head) / (page, slot, head)
+  int64_t qs[3], kds[3], vds[3];  // strides: (seq, node, head)
+  int64_t khead, vhead;           // the cache's: a head, and in pieces of 16 bytes a page and a slot
+  uint32_t kpage, kslot, vpage, vslot;
   int64_t table_stride, parents_stride;
   int32_t B, N, Hq, Hkv, D, S, P, M;  // S: page size, P: pages, M: table entries a sequence
   PageDiv div;
   float scale;
-  int32_t splits;  // parts of a sequence's keys
-  float* part;     // partial sums: [item][split][row][D], then {max, sum} [item][split][row]
+  int32_t per, most;  // tiles a part of a sequence's keys has at most, parts there are room for
+  float* part;        // [row tile][item][part][row][D], then {max, sum} [row tile][item][part][row]
 };
 
 constexpr int ATT_BLOCK = 256;
 constexpr int ATT_WAVES = ATT_BLOCK / 64;
 constexpr int ATT_TILE = 32;  // keys a wave works on at a time
+// The keys are cut so that about two workgroups a CU have work (more parts cost their joining: at 512 / 1024 / 2048
+// workgroups 64 trees of 5 nodes over up to 2237 positions took 42 / 49 / 44 us, 32 of 64 nodes over up to 16 k 610 /
+// 631 / 656), but no part gets below 16 tiles (with 8 one token over 237 positions took 10.8 us instead of 8.2).
+constexpr int ATT_WANT = 512, ATT_LEAST = 16;
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float LOWEST = -3.402823466e38f;  // the running maximum's start: exp2(-inf - LOWEST) is 0, not NaN
-
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 // The inputs' type in the matrix unit.  The weights w are rounded to it before the product with v.  In
-// fp16 they are held times 2^12 (the factor leaves with the division by their sum): a weight of 2^-37
-// of the largest keeps full precision then, so that many far keys are not lost against a near one.
+// fp16 they are held times 2^7 (the factor leaves with the division by their sum, and 2^SLACK times as much is
+// still in range): a weight of 2^-21 of the largest keeps full precision then, and those that are lost add up to
+// less than 2^-15 over 2^16 keys.
 template <typename T>
 struct Half;
 template <>
@@ -53,7 +58,7 @@ struct Half<bf16_t> {
 template <>
 struct Half<fp16_t> {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
-  static constexpr float bias = 12.f;
+  static constexpr float bias = 7.f;
   static __device__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
@@ -64,6 +69,27 @@ __device__ inline uint32_t pack2(float x, float y) {
   typedef T v2 __attribute__((ext_vector_type(2)));
   const v2 v = {(T)x, (T)y};
   return __builtin_bit_cast(uint32_t, v);
+}
+
+template <typename T>
+__device__ inline uint64_t pack4(f32x4 v) {
+  return (uint64_t)pack2<T>(v[2], v[3]) << 32 | pack2<T>(v[0], v[1]);
+}
+
+// Scores are compared as q k and scaled inside the exponent's multiply-add, exp2(q k c - max c), c = |scale| log2 e; a
+// negative scale turns the queries' signs.  A scale of 0 leaves a c that is too small to matter: -inf, what is not
+// there, stays -inf.
+__device__ inline float score_scale(float scale) { return fmaxf(fabsf(scale) * LOG2E, 1e-30f); }
+__device__ inline u32x4 signed_by(u32x4 q, float scale) {
+  const uint32_t s = scale < 0.f ? 0x80008000u : 0u;
+  return q ^ u32x4{s, s, s, s};
+}
+// a row that has seen no key has the maximum -inf: its weights are taken from 0, and are 0
+__device__ inline float at_least(float mx) { return mx == -INFINITY ? 0.f : mx; }
+
+// bytes from the cache's start to a slot
+__device__ inline uint64_t cache_row(int id, int slot, uint32_t page, uint32_t one) {
+  return ((uint64_t)(uint32_t)id * page + (uint64_t)(uint32_t)slot * one) << 4;
 }
 
 // over the four lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -112,7 +138,7 @@ __device__ inline void tree_paths(Tree& tr, int N, const int32_t* parents) {
   __syncthreads();
 }
 
-// keys of a sequence in tiles: the cache's, then the nodes'
+// a sequence's keys in tiles: the cache's, then the nodes'
 struct Span {
   int len, cache_tiles, tiles;
   bool bad;
@@ -128,18 +154,31 @@ __device__ inline Span span_of(const AttendArgs& a, int b, int tile) {
   return s;
 }
 
-// parts that a sequence of `tiles` tiles is really cut into, at least ATT_MIN tiles each
-constexpr int ATT_MIN = 16;
-#ifndef ATT_WANT
-#define ATT_WANT 1024
-#endif
-__host__ __device__ inline int parts_of(int tiles, int splits) { 
-  const int most = (tiles + ATT_MIN - 1) / ATT_MIN;
-  return splits < most ? splits : most;
+// values that are the same for the whole workgroup, as such
+__device__ inline int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// A sequence's tiles are cut into equal parts of at most `per`; a second kernel joins them.
+struct Share {
+  int parts, first, last;
+};
+__device__ inline Share share_of(const AttendArgs& a, int tiles, int part) {
+  Share s;
+  const int size = (tiles + (tiles + a.per - 1) / a.per - 1) / ((tiles + a.per - 1) / a.per);
+  s.parts = (tiles + size - 1) / size;
+  s.first = part * size;
+  s.last = min(s.first + size, tiles);
+  return s;
+}
+// a row's place among the parts
+__device__ inline int64_t part_row(const AttendArgs& a, int rt, int item, int part, int rows, int row) {
+  return (((int64_t)rt * a.B * a.Hkv + item) * a.most + part) * rows + row;
+}
+__device__ inline float* part_sums(const AttendArgs& a, int RT, int rows) {
+  return a.part + (int64_t)RT * a.B * a.Hkv * a.most * rows * a.D;
 }
 
-// A workgroup: RB blocks of 16 rows (row m: node m / G, head m % G of one kv head), one part of the keys;
-// its waves take the part's tiles of 32 keys in turn and join at the end.
+// A workgroup: RB blocks of 16 rows (row m: node m / G, head m % G of one kv head), one part of the keys; its
+// waves take the part's tiles of 32 keys in turn and join at the end.
 //
 // S^T = K Q^T and O^T = V^T P^T in the 16x16x32 matrix instruction: a lane then holds its own row's
 // weights (row = lane % 16), running maximum and sums, and the weights of four keys in a row are what the second
@@ -147,7 +186,7 @@ __host__ __device__ inline int parts_of(int tiles, int splits) {
 // registers, V through the wave's own LDS, where the transposing read turns it; the rows there are 32 bytes longer
 // than the head so that eight of them start in different banks.
 template <typename T, int KS, int RB>
-__global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
+__global__ __launch_bounds__(ATT_BLOCK, KS > 4 ? 1 : 2) void k_attend(AttendArgs a) {
   constexpr int DP = 32 * KS, DB = 2 * KS, LROW = DP * 2 + 32;
   constexpr int AREA = ATT_TILE * LROW;  // >= 16 rows of DP + 4 floats
   __shared__ __attribute__((aligned(16))) char lds[ATT_WAVES * AREA];
@@ -157,17 +196,18 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
   const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + RB * 16 - 1) / (RB * 16);
   // blocks go to the 8 dies in turn: the row tiles of one part stay on one die, one after the other
   const int die = blockIdx.x & 7, j8 = blockIdx.x >> 3;
-  const int rt = j8 % RT, item = (j8 / RT) * 8 + die;
-  if (item >= a.B * a.Hkv * a.splits) return;
-  const int split = item % a.splits, bh = item / a.splits, h = bh % a.Hkv, b = bh / a.Hkv;
+  const int rt = j8 % RT, work = (j8 / RT) * 8 + die;
+  if (work >= a.B * a.Hkv * a.most) return;
+  const int part = work % a.most, item = work / a.most, h = item % a.Hkv, b = item / a.Hkv;
   const Span sp = span_of(a, b, ATT_TILE);
-  const int parts = parts_of(sp.tiles, a.splits);
-  if (split >= parts) return;
-  const int per = (sp.tiles + parts - 1) / parts;
-  const int first = split * per, last = min(first + per, sp.tiles);
+  const Share sh = share_of(a, sp.tiles, part);
+  if (part >= sh.parts) return;
+  const int first = sh.first, last = sh.last;
+  char* area = lds + wave * AREA;
+  const float scale = score_scale(a.scale);
   const Pages pages = {a.table + b * a.table_stride, a.div, a.P, a.M};
-  const T* kc = (const T*)a.kc + h * a.kcs[2];
-  const T* vc = (const T*)a.vc + h * a.vcs[2];
+  const char* kc = (const char*)((const T*)a.kc + h * a.khead);
+  const char* vc = (const char*)((const T*)a.vc + h * a.vhead);
   const T* kd = (const T*)a.kd + b * a.kds[0] + h * a.kds[2];
   const T* vd = (const T*)a.vd + b * a.vds[0] + h * a.vds[2];
   bool bad = sp.bad;
@@ -193,7 +233,8 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
         bad = true;
         id[c] = 0;
       }
-      load(c, kc + id[c] * a.kcs[0] + slot[c] * a.kcs[1], vc + id[c] * a.vcs[0] + slot[c] * a.vcs[1]);
+      load(c, (const T*)(kc + cache_row(id[c], slot[c], a.kpage, a.kslot)),
+           (const T*)(vc + cache_row(id[c], slot[c], a.vpage, a.vslot)));
     }
   };
   auto fetch_nodes = [&](int base) {
@@ -216,20 +257,18 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
     for (int k = 0; k < KS; k++) {
       const int d = 32 * k + 8 * lq;
       const u32x4 zero = {0, 0, 0, 0};
-      qf[r][k] = m < M && d < a.D ? *(const u32x4*)(q + d) : zero;
+      qf[r][k] = m < M && d < a.D ? signed_by(*(const u32x4*)(q + d), a.scale) : zero;
     }
   }
   tree_paths(tr, a.N, a.parents + b * a.parents_stride);
 
-  const float scale = a.scale * LOG2E;
   float top[RB], sum[RB];
   f32x4 o[DB][RB];
   for (int r = 0; r < RB; r++) {
-    top[r] = LOWEST;
+    top[r] = -INFINITY;
     sum[r] = 0.f;
     for (int d = 0; d < DB; d++) o[d][r] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  char* area = lds + wave * AREA;
   auto step = [&](auto is_nodes, int base) {
     constexpr bool nodes = decltype(is_nodes)::value;
     bool odd = false;  // a node's value that is not finite
@@ -258,7 +297,6 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
     }
     u32x4 p[RB];
     for (int r = 0; r < RB; r++) {
-      for (int c = 0; c < 2; c++) s[c][r] *= scale;
       if constexpr (nodes) {
         const int m = (rt * RB + r) * 16 + l16;
         const uint32_t set = m < M ? tr.anc[m / G][base / 32] : 0;
@@ -274,15 +312,16 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
       for (int c = 0; c < 2; c++)
         for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[c][r][i]);
       mx = quad_max(mx);
+      const float from = at_least(mx);
       if (__any(mx > top[r])) {
-        const float f = __builtin_amdgcn_exp2f(top[r] - mx);
+        const float f = __builtin_amdgcn_exp2f((top[r] - from) * scale);
         top[r] = mx;
         sum[r] *= f;
         for (int d = 0; d < DB; d++) o[d][r] *= f;
       }
-      const float off = Half<T>::bias - mx;
+      const float off = fmaf(-from, scale, Half<T>::bias);
       for (int c = 0; c < 2; c++)
-        for (int i = 0; i < 4; i++) s[c][r][i] = __builtin_amdgcn_exp2f(s[c][r][i] + off);
+        for (int i = 0; i < 4; i++) s[c][r][i] = __builtin_amdgcn_exp2f(fmaf(s[c][r][i], scale, off));
       sum[r] += ((s[0][r][0] + s[0][r][1]) + (s[0][r][2] + s[0][r][3])) +
                 ((s[1][r][0] + s[1][r][1]) + (s[1][r][2] + s[1][r][3]));
       for (int c = 0; c < 2; c++)
@@ -293,7 +332,6 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
       for (int c = 0; c < 2; c++) {
         const char* at = area + (16 * c + 4 * lq + (l16 >> 2)) * LROW + (16 * d + 4 * (l16 & 3)) * 2;
         const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
         const u32x2 y = __builtin_bit_cast(u32x2, x);
         v[2 * c] = y[0];
         v[2 * c + 1] = y[1];
@@ -319,7 +357,7 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
           float dot = 0.f;
 #pragma unroll 1
           for (int e = 0; e < a.D; e++) dot = fmaf((float)q[e], (float)k[e], dot);
-          const float w = __builtin_amdgcn_exp2f(dot * scale + Half<T>::bias - top[r]);
+          const float w = __builtin_amdgcn_exp2f(fmaf((a.scale < 0.f ? -dot : dot) - at_least(top[r]), scale, Half<T>::bias));
 #pragma unroll 1
           for (int d = 4 * lq; d < a.D; d += 16) {
             if (!not_finite<T>(*(const u32x4*)(v + d / 8 * 8))) continue;
@@ -351,7 +389,6 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
       ml[1][wave][r * 16 + l16] = sum[r];
     }
   }
-  const int bhr = bh * RT + rt;
   for (int r = 0; r < RB; r++) {
     __syncthreads();
     float* mine = (float*)area + l16 * (DP + 4) + 4 * lq;
@@ -360,29 +397,29 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
     for (int e = t; e < 16 * DP / 4; e += ATT_BLOCK) {
       const int row = e / (DP / 4), d = e % (DP / 4) * 4, m = (rt * RB + r) * 16 + row;
       if (m >= M || d >= a.D) continue;
-      float mx = LOWEST;
+      float mx = -INFINITY;
       for (int w = 0; w < ATT_WAVES; w++) mx = fmaxf(mx, ml[0][w][r * 16 + row]);
+      const float from = at_least(mx);
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       float total = 0.f;
       for (int w = 0; w < ATT_WAVES; w++) {
-        const float f = __builtin_amdgcn_exp2f(ml[0][w][r * 16 + row] - mx);
+        const float f = __builtin_amdgcn_exp2f((ml[0][w][r * 16 + row] - from) * scale);
         total += f * ml[1][w][r * 16 + row];
         acc += f * *(const f32x4*)((const float*)(lds + w * AREA) + row * (DP + 4) + d);
       }
-      if (parts == 1) {
-        const int n = m / G;
+      const int n = m / G;
+      const bool here = tr.anc[n][n / 32] >> (n % 32) & 1;
+      if (sh.parts == 1) {
         T* out = (T*)a.out + (((int64_t)b * a.N + n) * a.Hq + h * G + m - n * G) * a.D + d;
-        const bool here = tr.anc[n][n / 32] >> (n % 32) & 1;
-        const float f = 1.f / total;
-        uint32_t w[2] = {pack2<T>(acc[0] * f, acc[1] * f), pack2<T>(acc[2] * f, acc[3] * f)};
-        *(uint64_t*)out = here ? (uint64_t)w[1] << 32 | w[0] : 0;
+        *(uint64_t*)out = here ? pack4<T>(acc * (1.f / total)) : 0;
       } else {
-        const int64_t at = ((int64_t)bhr * a.splits + split) * (RB * 16) + r * 16 + row;
-        *(f32x4*)(a.part + at * a.D + d) = acc;
+        const int64_t at = part_row(a, rt, item, part, RB * 16, r * 16 + row);
+        const f32x4 none = {0.f, 0.f, 0.f, 0.f};  // an absent row's parts: a sum of 0
+        *(f32x4*)(a.part + at * a.D + d) = here ? acc : none;
         if (d == 0) {
-          float* p = a.part + (int64_t)a.B * a.Hkv * RT * a.splits * (RB * 16) * a.D + 2 * at;
-          p[0] = mx;
-          p[1] = total;
+          float* p = part_sums(a, RT, RB * 16) + 2 * at;
+          p[0] = here ? mx : -INFINITY;
+          p[1] = here ? total : 0.f;
         }
       }
     }
@@ -400,6 +437,7 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend(AttendArgs a) {
 // 128 bytes: c ^ 4 (r / 2 & 1)).
 constexpr int WIDE_TILE = 64;
 constexpr int WIDE_ROWS = 128;
+constexpr float SLACK = 8.f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -428,6 +466,15 @@ __device__ inline void to_lds(const void* p, uint32_t at) {
                : "memory");
 }
 
+// LDS by its byte address; `plus` goes into the instruction
+template <typename V>
+__device__ inline V lds_read(uint32_t at, int plus) {
+  return *(const __attribute__((address_space(3))) V*)(uintptr_t)(at + plus);
+}
+__device__ inline u32x2 lds_read_tr(uint32_t at, int plus) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4*)(uintptr_t)(at + plus)));
+}
 __device__ inline void wait_loads() {
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), as the compiler counts it too
   asm volatile("" ::: "memory");
@@ -440,141 +487,265 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
   constexpr int CH = DP / 8, KSTEPS = DP / 16, DB = DP / 32;
   constexpr int TILE_BYTES = WIDE_TILE * DP * 2, PER = WIDE_TILE * CH / ATT_BLOCK;  // pieces a thread moves
   constexpr int RPI = ATT_BLOCK / CH;                                               // rows between them
-  __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];                 // K, V; twice
+  constexpr uint32_t VBUF = 2 * TILE_BYTES;
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];  // K of two tiles, V of two
+  __shared__ uint64_t offs[4][2][WIDE_TILE];                         // the rows' places in the cache: tile % 4, K or V
   __shared__ Tree tr;
   __shared__ int odd_;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, hh = lane >> 5;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  const float scale = score_scale(a.scale);
   const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + WIDE_ROWS - 1) / WIDE_ROWS;
   const int die = blockIdx.x & 7, j8 = blockIdx.x >> 3;
-  const int rt = j8 % RT, item = (j8 / RT) * 8 + die;
-  if (item >= a.B * a.Hkv * a.splits) return;
-  const int split = item % a.splits, bh = item / a.splits, h = bh % a.Hkv, b = bh / a.Hkv;
+  const int rt = uni(j8 % RT), work = uni((j8 / RT) * 8 + die);
+  if (work >= a.B * a.Hkv * a.most) return;
+  const int part = uni(work % a.most), item = uni(work / a.most), h = uni(item % a.Hkv), b = uni(item / a.Hkv);
   const Span sp = span_of(a, b, WIDE_TILE);
-  const int parts = parts_of(sp.tiles, a.splits);
-  if (split >= parts) return;
-  const int per = (sp.tiles + parts - 1) / parts;
-  const int first = split * per, last = min(first + per, sp.tiles);
-  const Pages pages = {a.table + b * a.table_stride, a.div, a.P, a.M};
-  const T* kc = (const T*)a.kc + h * a.kcs[2];
-  const T* vc = (const T*)a.vc + h * a.vcs[2];
-  const T* kd = (const T*)a.kd + b * a.kds[0] + h * a.kds[2];
-  const T* vd = (const T*)a.vd + b * a.vds[0] + h * a.vds[2];
-  bool bad = sp.bad;
-  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  const Share sh = share_of(a, sp.tiles, part);
+  if (part >= sh.parts) return;
+  const int m = rt * WIDE_ROWS + wave * 32 + l32, node = m / G;
+  const bool rows = rt * WIDE_ROWS + uni(wave) * 32 < M;  // (the wave has any)
 
-  // thread t moves piece t % CH (as it lies in LDS) of the rows t / CH + RPI i
-  const int prow = t / CH, pc = t % CH;
+  // where this lane's operands lie in a tile: K's piece 2 k + hh of row l32, V's four keys of 16 channels
   auto kswz = [](int row) { return row & 7 & (CH - 1); };
   auto vswz = [](int row) { return CH >= 16 ? (row & 3) << 2 : CH == 8 ? (row >> 1 & 1) << 2 : 0; };
-  int id[PER], slot[PER];
-  auto find = [&](int tile) {
-    for (int i = 0; i < PER; i++) id[i] = page_entry(pages, min(tile * WIDE_TILE + prow + RPI * i, sp.len - 1), slot[i]);
-  };
-  auto stage = [&](int buf) {
-    const uint32_t k = lds_at + buf * 2 * TILE_BYTES + wave * 1024;  // the wave's 64 pieces in a row
-    for (int i = 0; i < PER; i++) {
-      if (!good_page(pages, id[i])) {  // reads page 0, and the sequence's rows become NaN
-        bad = true;
-        id[i] = 0;
+  uint32_t koff[KSTEPS], voff[DB];
+  for (int k = 0; k < KSTEPS; k++) koff[k] = lds_at + (l32 * CH + ((2 * k + hh) ^ kswz(l32))) * 16;
+  for (int d = 0; d < DB; d++) {
+    const int row = 4 * hh + (lane >> 2 & 3), col = 32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+    voff[d] = lds_at + VBUF + (row * CH + ((col / 8) ^ vswz(row))) * 16 + (col & 4) * 2;
+  }
+  // thread t moves piece t % CH (as it lies in LDS) of the rows t / CH + RPI i
+  const int prow = t / CH, pc = t % CH;
+
+  {
+    const int last = uni(sh.last), cached = min(last, uni(sp.cache_tiles));
+    int tile = uni(sh.first);
+    bool bad = sp.bad;
+    float top = -INFINITY, sum = 0.f;  // the row's reference and its sum of weights
+    f32x16 o[DB];
+    for (int d = 0; d < DB; d++)
+      for (int i = 0; i < 16; i++) o[d][i] = 0.f;
+    u32x4 qf[KSTEPS];
+
+    auto scores = [&](f32x16* s, uint32_t buf) {
+      for (int c = 0; c < 2; c++) {
+        for (int i = 0; i < 16; i++) s[c][i] = 0.f;
+        for (int k = 0; k < KSTEPS; k++)
+          s[c] = mfma32(lds_read<u32x4>(koff[k] + buf, c * 32 * CH * 16), qf[k], s[c], T());
       }
-      const int row = prow + RPI * i, ck = (pc ^ kswz(row)) * 8, cv = (pc ^ vswz(row)) * 8;
-      const T* kp = kc + id[i] * a.kcs[0] + slot[i] * a.kcs[1] + ck;
-      const T* vp = vc + id[i] * a.vcs[0] + slot[i] * a.vcs[1] + cv;
-      to_lds(ck < a.D ? (const void*)kp : &att_zero, k + i * ATT_BLOCK * 16);
-      to_lds(cv < a.D ? (const void*)vp : &att_zero, k + TILE_BYTES + i * ATT_BLOCK * 16);
-    }
-  };
-  const int cached = min(last, sp.cache_tiles);
-  int tile = first;
-  if (tile < cached) {
-    find(tile);
-    wait_loads();
-    stage(0);
-    if (tile + 1 < cached) find(tile + 1);
-  }
-  const int m = rt * WIDE_ROWS + wave * 32 + l32, node = m / G;
-  const bool rows = rt * WIDE_ROWS + wave * 32 < M;  // (the wave has any)
-  u32x4 qf[KSTEPS];
-  const T* q = (const T*)a.q + b * a.qs[0] + node * a.qs[1] + (h * G + m - node * G) * a.qs[2];
-  for (int k = 0; k < KSTEPS; k++) {
-    const int d = 16 * k + 8 * hh;
-    qf[k] = m < M && d < a.D ? *(const u32x4*)(q + d) : att_zero;
-  }
-  if (t == 0) odd_ = 0;
-  tree_paths(tr, a.N, a.parents + b * a.parents_stride);
+    };
+    // The weights are taken from a reference that follows the maximum: it moves when a score is over it by 2^8 in the
+    // weights, so that the sums are seldom scaled anew.
+    auto follow = [&](const f32x16* s) {
+      float mx = top;
+      for (int c = 0; c < 2; c++)
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[c][i]);
+      mx = pair_max(mx);
+      if (__any((mx - top) * scale > SLACK)) {
+        const float f = __builtin_amdgcn_exp2f((top - at_least(mx)) * scale);
+        top = mx;
+        sum *= f;
+        for (int d = 0; d < DB; d++) o[d] *= f;
+      }
+    };
+    auto weigh = [&](const f32x16* s, u32x4* p) {
+      const float off = fmaf(-at_least(top), scale, Half<T>::bias);
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; c < 2; c++)
+        for (int i = 0; i < 16; i += 2) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[c][i], scale, off));
+          const float y = __builtin_amdgcn_exp2f(fmaf(s[c][i + 1], scale, off));
+          part[i / 2 % 4] += x + y;
+          p[2 * c + i / 8][i / 2 % 4] = pack2<T>(x, y);
+        }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+    };
+    auto product = [&](const u32x4* p, uint32_t buf) {
+      for (int st = 0; st < 4; st++)  // 16 keys: the lane's are 16 st + 4 hh + {0..3, 8..11}
+        for (int d = 0; d < DB; d++) {
+          const u32x2 x = lds_read_tr(voff[d] + buf, 16 * st * CH * 16), y = lds_read_tr(voff[d] + buf, (16 * st + 8) * CH * 16);
+          o[d] = mfma32(u32x4{x[0], x[1], y[0], y[1]}, p[st], o[d], T());
+        }
+    };
 
-  const float scale = a.scale * LOG2E;
-  float top = LOWEST, sum = 0.f;
-  f32x16 o[DB];
-  for (int d = 0; d < DB; d++)
-    for (int i = 0; i < 16; i++) o[d][i] = 0.f;
-
-  auto step = [&](auto is_nodes, int base, int buf) {
-    constexpr bool nodes = decltype(is_nodes)::value;
-    const char* kt = lds + buf * 2 * TILE_BYTES;
-    const char* vt = kt + TILE_BYTES;
-    f32x16 s[2];
-    for (int c = 0; c < 2; c++) {
-      for (int i = 0; i < 16; i++) s[c][i] = 0.f;
-      const int row = 32 * c + l32;
+    {
+      const int len = uni(sp.len);
+      if (t == 0) odd_ = 0;
+      const Pages pages = {a.table + b * a.table_stride, a.div, a.P, a.M};
+      const char* kc = (const char*)((const T*)a.kc + h * a.khead);
+      const char* vc = (const char*)((const T*)a.vc + h * a.vhead);
+      // A row's place is worked out once, by one of 32 lanes a wave, and goes to the others through LDS; its table
+      // entry is loaded a tile before that, and looked at only then: nothing waits for it.
+      const int orow = wave * 16 + (lane & 15), okv = lane >> 4 & 1;
+      int entry = 0, slot = 0;
+      auto find = [&](int tile) { entry = page_entry(pages, min(tile * WIDE_TILE + orow, len - 1), slot); };
+      auto locate = [&](int tile) {
+        if (!good_page(pages, entry)) {  // reads page 0, and the sequence's rows become NaN
+          bad = true;
+          entry = 0;
+        }
+        const uint64_t at = okv ? cache_row(entry, slot, a.vpage, a.vslot) : cache_row(entry, slot, a.kpage, a.kslot);
+        if (lane < 32) offs[tile & 3][okv][orow] = at;
+      };
+      auto stage = [&](int tile, int kv) {
+        const uint32_t to = lds_at + kv * VBUF + (tile & 1) * TILE_BYTES + wave * 1024;  // the wave's 64 pieces in a row
+        for (int i = 0; i < PER; i++) {
+          const int row = prow + RPI * i, c = (pc ^ (kv ? vswz(row) : kswz(row))) * 8;
+          const char* p = (kv ? vc : kc) + offs[tile & 3][kv][row] + c * 2;
+          to_lds(c < a.D ? (const void*)p : &att_zero, to + i * ATT_BLOCK * 16);
+        }
+      };
+      if (tile < cached) {
+        find(tile);
+        locate(tile);
+        find(tile + 1);
+        locate(tile + 1);
+        find(tile + 2);
+        __syncthreads();
+        wait_loads();
+        stage(tile, 0);
+        stage(tile, 1);
+        if (tile + 1 < cached) stage(tile + 1, 0);
+        locate(tile + 2);
+        find(tile + 3);
+      }
+      const T* q = (const T*)a.q + b * a.qs[0] + node * a.qs[1] + (h * G + m - node * G) * a.qs[2];
       for (int k = 0; k < KSTEPS; k++) {
-        const u32x4 kf = *(const u32x4*)(kt + (row * CH + ((2 * k + hh) ^ kswz(row))) * 16);
-        s[c] = mfma32(kf, qf[k], s[c], T());
+        const int d = 16 * k + 8 * hh;
+        qf[k] = m < M && d < a.D ? signed_by(*(const u32x4*)(q + d), a.scale) : att_zero;
+      }
+      tree_paths(tr, a.N, a.parents + b * a.parents_stride);
+
+      // The cache's tiles: a tile's scores are worked out while the weights of the one before it are, in the matrix
+      // unit and beside it.  So K comes two tiles ahead and V one.
+      f32x16 s[2];
+      auto hide = [&](int tile) {  // key 32 c + 8 (i / 4) + 4 hh + i % 4 of the tile
+        if ((tile + 1) * WIDE_TILE <= len) return;
+        for (int c = 0; c < 2; c++)
+          for (int i = 0; i < 16; i++)
+            if (tile * WIDE_TILE + 32 * c + 8 * (i / 4) + 4 * hh + i % 4 >= len) s[c][i] = -INFINITY;
+      };
+      if (tile < cached) {
+        wait_loads();
+        __syncthreads();
+        if (rows) {
+          scores(s, (tile & 1) * TILE_BYTES);
+          hide(tile);
+          follow(s);
+        }
+      }
+      for (; tile + 1 < cached; tile++) {
+        wait_loads();     // this wave's pieces are in LDS
+        __syncthreads();  // everyone's are; what the last tile was read from is free
+        locate(tile + 3);
+        find(tile + 4);
+        if (tile + 2 < cached) stage(tile + 2, 0);
+        stage(tile + 1, 1);
+        if (!rows) continue;
+        // In eight steps, each with products beside the exponentials of another step's weights.
+        const uint32_t vb = (tile & 1) * TILE_BYTES, kb = vb ^ TILE_BYTES;
+        constexpr int KC = KSTEPS / 4;
+        const float off = fmaf(-at_least(top), scale, Half<T>::bias);
+        float part[2] = {0.f, 0.f};
+        f32x16 n[2];
+        u32x4 p[4];
+        auto keys = [&](int i) {
+          for (int k = i * KC; k < (i + 1) * KC; k++)
+            for (int c = 0; c < 2; c++) {
+              const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+              n[c] = mfma32(lds_read<u32x4>(koff[k] + kb, c * 32 * CH * 16), qf[k], k ? n[c] : zero, T());
+            }
+        };
+        auto values = [&](int st) {
+          for (int d = 0; d < DB; d++) {
+            const u32x2 x = lds_read_tr(voff[d] + vb, 16 * st * CH * 16), y = lds_read_tr(voff[d] + vb, (16 * st + 8) * CH * 16);
+            o[d] = mfma32(u32x4{x[0], x[1], y[0], y[1]}, p[st], o[d], T());
+          }
+        };
+        auto expo = [&](int st, int half) {
+          for (int e = 0; e < 4; e += 2) {
+            const int i = 8 * (st & 1) + 4 * half + e;
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[st / 2][i], scale, off));
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[st / 2][i + 1], scale, off));
+            part[half] += x + y;
+            p[st][2 * half + e / 2] = pack2<T>(x, y);
+          }
+        };
+        auto then = []() { __builtin_amdgcn_sched_barrier(0); };
+        expo(0, 0), keys(0);
+        then();
+        expo(0, 1), keys(1);
+        then();
+        expo(1, 0), values(0);
+        then();
+        expo(1, 1), keys(2);
+        then();
+        expo(2, 0), values(1);
+        then();
+        expo(2, 1), keys(3);
+        then();
+        expo(3, 0), expo(3, 1), values(2);
+        then();
+        values(3);
+        sum += part[0] + part[1];
+        s[0] = n[0];
+        s[1] = n[1];
+        hide(tile + 1);
+        follow(s);
+      }
+      if (tile < cached) {
+        wait_loads();
+        __syncthreads();
+        if (rows) {
+          u32x4 p[4];
+          weigh(s, p);
+          product(p, (tile & 1) * TILE_BYTES);
+        }
+        tile++;
       }
     }
-    // key 32 c + 8 (i / 4) + 4 hh + i % 4 of the tile
-    for (int c = 0; c < 2; c++) s[c] *= scale;
-    if constexpr (nodes) {
+
+    // the tree's own keys, one tile after the other
+    for (; tile < last; tile++) {
+      const int base = (tile - uni(sp.cache_tiles)) * WIDE_TILE;
+      const T* kd = (const T*)a.kd + b * a.kds[0] + h * a.kds[2];
+      const T* vd = (const T*)a.vd + b * a.vds[0] + h * a.vds[2];
+      __syncthreads();
+      // through registers: a value that is not finite would reach every row as 0 times itself; it goes in as 0 and is
+      // added on its own path
+      for (int i = 0; i < PER; i++) {
+        const int row = prow + RPI * i, n = min(base + row, a.N - 1);
+        const int ck = (pc ^ kswz(row)) * 8, cv = (pc ^ vswz(row)) * 8;
+        const u32x4 k = ck < a.D ? *(const u32x4*)(kd + n * a.kds[1] + ck) : att_zero;
+        u32x4 v = cv < a.D ? *(const u32x4*)(vd + n * a.vds[1] + cv) : att_zero;
+        if (not_finite<T>(v)) {
+          v = att_zero;
+          odd_ = 1;
+        }
+        *(u32x4*)(lds + (t + ATT_BLOCK * i) * 16) = k;
+        *(u32x4*)(lds + VBUF + (t + ATT_BLOCK * i) * 16) = v;
+      }
+      __syncthreads();
+      if (!rows) continue;
+      f32x16 s[2];
+      u32x4 p[4];
+      scores(s, 0);
       for (int c = 0; c < 2; c++) {
         const uint32_t set = m < M ? tr.anc[node][base / 32 + c] : 0;
         for (int i = 0; i < 16; i++)
           if (!(set >> (8 * (i / 4) + 4 * hh + i % 4) & 1)) s[c][i] = -INFINITY;
       }
-    } else if (base + WIDE_TILE > sp.len) {
-      for (int c = 0; c < 2; c++)
-        for (int i = 0; i < 16; i++)
-          if (base + 32 * c + 8 * (i / 4) + 4 * hh + i % 4 >= sp.len) s[c][i] = -INFINITY;
-    }
-    float mx = top;
-    for (int c = 0; c < 2; c++)
-      for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[c][i]);
-    mx = pair_max(mx);
-    if (__any(mx > top)) {
-      const float f = __builtin_amdgcn_exp2f(top - mx);
-      top = mx;
-      sum *= f;
-      for (int d = 0; d < DB; d++) o[d] *= f;
-    }
-    const float off = Half<T>::bias - mx;
-    u32x4 p[4];
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < 2; c++)
-      for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(s[c][i] + off), y = __builtin_amdgcn_exp2f(s[c][i + 1] + off);
-        part[i / 2 % 4] += x + y;
-        p[2 * c + i / 8][i / 2 % 4] = pack2<T>(x, y);
-      }
-    sum += (part[0] + part[1]) + (part[2] + part[3]);
-    for (int st = 0; st < 4; st++)  // 16 keys: the lane's are 16 st + 4 hh + {0..3, 8..11}
-      for (int d = 0; d < DB; d++) {
-        u32x4 v;
-        for (int c = 0; c < 2; c++) {
-          const int row = 16 * st + 8 * c + 4 * hh + (lane >> 2 & 3), col = 32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-          const char* at = vt + (row * CH + ((col / 8) ^ vswz(row))) * 16 + (col & 4) * 2;
-          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-          typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-          const u32x2 y = __builtin_bit_cast(u32x2, x);
-          v[2 * c] = y[0];
-          v[2 * c + 1] = y[1];
-        }
-        o[d] = mfma32(v, p[st], o[d], T());
-      }
-    if constexpr (nodes) {
-      if (!odd_) return;
-      // the sums of what went in as 0, in the LDS that the tiles do not use now
-      float* mine = (float*)(lds + 2 * TILE_BYTES) + ((wave * 32 + l32) * DP / 2);
+      follow(s);
+      weigh(s, p);
+      product(p, 0);
+      if (!odd_) continue;
+      // the sums of what went in as 0 (the finite values of its pieces with their weights), half the channels at a time,
+      // in the LDS that the tile does not use
+#pragma unroll
       for (int half = 0; half < 2; half++) {
-        const int d0 = half * (DP / 2);
+        const int slice = wave * 32 + l32, d0 = half * (DP / 2);
+        float* mine = (float*)(lds + (slice < WIDE_ROWS / 2 ? TILE_BYTES : VBUF + TILE_BYTES)) + slice % (WIDE_ROWS / 2) * (DP / 2);
 #pragma unroll 1
         for (int d = 4 * hh; d < DP / 2; d += 8) *(f32x4*)(mine + d) = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
@@ -582,10 +753,11 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
           if (m >= M || !(tr.anc[node][(base + j) / 32] >> (j % 32) & 1)) continue;
           const T* v = vd + (base + j) * a.vds[1];
           const T* k = kd + (base + j) * a.kds[1];
+          const T* q = (const T*)a.q + b * a.qs[0] + node * a.qs[1] + (h * G + m - node * G) * a.qs[2];
           float dot = 0.f;
 #pragma unroll 1
           for (int e = 0; e < a.D; e++) dot = fmaf((float)q[e], (float)k[e], dot);
-          const float w = __builtin_amdgcn_exp2f(dot * scale + Half<T>::bias - top);
+          const float w = __builtin_amdgcn_exp2f(fmaf((a.scale < 0.f ? -dot : dot) - at_least(top), scale, Half<T>::bias));
 #pragma unroll 1
           for (int d = 4 * hh; d < DP / 2 && d0 + d < a.D; d += 8) {
             if (!not_finite<T>(*(const u32x4*)(v + (d0 + d) / 8 * 8))) continue;
@@ -610,93 +782,83 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
         wave_order();
       }
     }
-  };
-  for (int buf = 0; tile < cached; tile++, buf ^= 1) {
-    wait_loads();     // this wave's pieces of the tile are in LDS
-    __syncthreads();  // everyone's are, and the other buffer is free
-    if (tile + 1 < cached) {
-      stage(buf ^ 1);
-      if (tile + 2 < cached) find(tile + 2);
-    }
-    if (rows) step(std::false_type(), tile * WIDE_TILE, buf);
-  }
-  for (; tile < last; tile++) {
-    // nodes go through registers: a value that is not finite goes in as 0 and is added on its own path
-    const int base = (tile - sp.cache_tiles) * WIDE_TILE;
-    __syncthreads();
-    for (int i = 0; i < PER; i++) {
-      const int row = prow + RPI * i, n = min(base + row, a.N - 1);
-      const int ck = (pc ^ kswz(row)) * 8, cv = (pc ^ vswz(row)) * 8;
-      const u32x4 k = ck < a.D ? *(const u32x4*)(kd + n * a.kds[1] + ck) : att_zero;
-      u32x4 v = cv < a.D ? *(const u32x4*)(vd + n * a.vds[1] + cv) : att_zero;
-      if (not_finite<T>(v)) {
-        v = att_zero;
-        odd_ = 1;
-      }
-      *(u32x4*)(lds + (t + ATT_BLOCK * i) * 16) = k;
-      *(u32x4*)(lds + TILE_BYTES + (t + ATT_BLOCK * i) * 16) = v;
-    }
-    __syncthreads();
-    if (rows) step(std::true_type(), base, 0);
-  }
 
-  sum += __shfl_xor(sum, 32);
-  const bool any_bad = __syncthreads_or(bad);
-  if (m >= M) return;
-  if (any_bad) sum = NAN;
-  const int64_t at = ((int64_t)(bh * RT + rt) * a.splits + split) * WIDE_ROWS + wave * 32 + l32;
-  const bool here = tr.anc[node][node / 32] >> (node % 32) & 1;
-  const float f = 1.f / sum;
-  T* out = (T*)a.out + (((int64_t)b * a.N + node) * a.Hq + h * G + m - node * G) * a.D;
-  if (parts > 1 && hh == 0) {
-    float* ml = a.part + (int64_t)a.B * a.Hkv * RT * a.splits * WIDE_ROWS * a.D + 2 * at;
-    ml[0] = top;
-    ml[1] = sum;
-  }
-  for (int d = 0; d < DB; d++)
-    for (int i = 0; i < 4; i++) {
-      const int x = 32 * d + 8 * i + 4 * hh;
-      if (x >= a.D) continue;
-      if (parts > 1) {
-        *(f32x4*)(a.part + at * a.D + x) = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-      } else {
-        const uint32_t w[2] = {pack2<T>(o[d][4 * i] * f, o[d][4 * i + 1] * f), pack2<T>(o[d][4 * i + 2] * f, o[d][4 * i + 3] * f)};
-        *(uint64_t*)(out + x) = here ? (uint64_t)w[1] << 32 | w[0] : 0;
+    sum += __shfl_xor(sum, 32);
+    if (__syncthreads_or(bad)) sum = NAN;
+    if (m < M) {
+      const int64_t at = part_row(a, rt, item, part, WIDE_ROWS, wave * 32 + l32);
+      const bool here = tr.anc[node][node / 32] >> (node % 32) & 1;
+      const float f = 1.f / sum;
+      T* out = (T*)a.out + (((int64_t)b * a.N + node) * a.Hq + h * G + m - node * G) * a.D;
+      if (sh.parts > 1 && hh == 0) {
+        float* ml = part_sums(a, RT, WIDE_ROWS) + 2 * at;
+        ml[0] = here ? top : -INFINITY;
+        ml[1] = here ? sum : 0.f;
       }
+      for (int d = 0; d < DB; d++)
+        for (int i = 0; i < 4; i++) {
+          const int x = 32 * d + 8 * i + 4 * hh;
+          if (x >= a.D) continue;
+          const f32x4 y = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}, none = {0.f, 0.f, 0.f, 0.f};
+          if (sh.parts > 1)  // (an absent row's parts: a sum of 0)
+            *(f32x4*)(a.part + at * a.D + x) = here ? y : none;
+          else
+            *(uint64_t*)(out + x) = here ? pack4<T>(y * f) : 0;
+        }
     }
+  }
 }
 
-// joins the parts of a sequence: one wave a row
-template <typename T>
+// Joins the parts: D / 4 threads a row, BY of them over its parts, eight parts in flight each.  Rows of sequences with
+// one part were written already.
+template <typename T, int BY>
 __global__ __launch_bounds__(ATT_BLOCK) void k_attend_join(AttendArgs a, int rows, int tile) {
-  const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + rows - 1) / rows;
-  const int64_t x = (int64_t)blockIdx.x * ATT_WAVES + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (x >= (int64_t)a.B * a.Hkv * M) return;
-  const int m = (int)(x % M), bh = (int)(x / M), h = bh % a.Hkv, b = bh / a.Hkv, n = m / G;
-  const int parts = parts_of(span_of(a, b, tile).tiles, a.splits);
-  if (parts == 1) return;  // (written already)
-  // present: the walk to the root
-  const int32_t* par = a.parents + b * a.parents_stride;
-  const bool here = draft_depth(par, n) >= 0;
-  const int64_t at = ((int64_t)bh * RT + m / rows) * a.splits * rows + m % rows;
-  const float* ml = a.part + (int64_t)a.B * a.Hkv * RT * a.splits * rows * a.D;
-  float mx = LOWEST;
-  for (int s = 0; s < parts; s++) mx = fmaxf(mx, ml[2 * (at + (int64_t)s * rows)]);
-  T* out = (T*)a.out + (((int64_t)b * a.N + n) * a.Hq + h * G + m - n * G) * a.D;
-  for (int d = lane * 4; d < a.D; d += 256) {
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    float total = 0.f;
-    for (int s = 0; s < parts; s++) {
-      const int64_t r = at + (int64_t)s * rows;
-      const float f = __builtin_amdgcn_exp2f(ml[2 * r] - mx);
-      total += f * ml[2 * r + 1];
-      acc += f * *(const f32x4*)(a.part + r * a.D + d);
+  __shared__ f32x4 acc_[BY > 1 ? ATT_BLOCK : 1];
+  __shared__ float ml_[2][BY > 1 ? ATT_BLOCK : 1];
+  const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + rows - 1) / rows, t = threadIdx.x;
+  const int q = a.D / 4, each = ATT_BLOCK / (q * BY);  // rows a workgroup
+  const int r = t / (q * BY), by = t / q % BY, d = t % q * 4;
+  const int64_t x = (int64_t)blockIdx.x * each + r;
+  const bool on = r < each && x < (int64_t)a.B * a.Hkv * M;
+  const int m = on ? (int)(x % M) : 0, bh = on ? (int)(x / M) : 0, h = bh % a.Hkv, b = bh / a.Hkv, n = m / G;
+  const int parts = on ? share_of(a, span_of(a, b, tile).tiles, 0).parts : 1;
+  const float scale = score_scale(a.scale);
+  const int64_t base = part_row(a, m / rows, bh, 0, rows, m % rows);
+  const float* ml = part_sums(a, RT, rows);
+  float mx = -INFINITY, total = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](float m2, float l2, f32x4 v) {
+    const float up = fmaxf(mx, m2), from = at_least(up);
+    const float f = __builtin_amdgcn_exp2f((mx - from) * scale), g = __builtin_amdgcn_exp2f((m2 - from) * scale);
+    total = total * f + l2 * g;
+    acc = acc * f + v * g;
+    mx = up;
+  };
+  if (parts > 1)
+    for (int k = by; k < parts; k += 8 * BY) {
+      float m2[8], l2[8];
+      f32x4 v[8];
+      for (int j = 0; j < 8; j++) {
+        const int e = min(k + j * BY, parts - 1);
+        const int64_t at = base + (int64_t)e * rows;
+        m2[j] = ml[2 * at];
+        l2[j] = ml[2 * at + 1];
+        v[j] = *(const f32x4*)(a.part + at * a.D + d);
+      }
+      for (int j = 0; j < 8; j++)
+        if (k + j * BY < parts) add(m2[j], l2[j], v[j]);
     }
-    const float f = 1.f / total;
-    uint32_t w[2] = {pack2<T>(acc[0] * f, acc[1] * f), pack2<T>(acc[2] * f, acc[3] * f)};
-    *(uint64_t*)(out + d) = here ? (uint64_t)w[1] << 32 | w[0] : 0;
+  if constexpr (BY > 1) {
+    acc_[t] = acc;
+    ml_[0][t] = mx;
+    ml_[1][t] = total;
+    __syncthreads();
+    if (by || r >= each) return;
+    for (int k = 1; k < BY; k++) add(ml_[0][t + k * q], ml_[1][t + k * q], acc_[t + k * q]);
   }
+  if (parts == 1) return;
+  T* out = (T*)a.out + (((int64_t)b * a.N + n) * a.Hq + h * G + m - n * G) * a.D + d;
+  *(uint64_t*)out = total == 0.f ? 0 : pack4<T>(acc * (1.f / total));
 }
 
 }  // namespace gb

@@ -25,7 +25,7 @@ struct {
 } lib;
 PyObject* geobpe_error;  // geobpe._native.GeoBPEError
 
-constexpr int64_t MAX_NODES = 128, MAX_VOCAB = 1 << 22, MAX_POSITIONS = 0x7fffffc0;
+constexpr int64_t MAX_NODES = 128, MAX_VOCAB = 1 << 22, MAX_POSITIONS = 0x7ffff000;
 
 struct Refused {};  // thrown with the Python error set
 

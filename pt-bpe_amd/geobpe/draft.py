@@ -25,7 +25,7 @@ from . import _native
 
 MAX_NODES = 128
 MAX_VOCAB = 1 << 22
-MAX_POSITIONS = (1 << 31) - 64
+MAX_POSITIONS = (1 << 31) - 4096
 
 _HALF = (torch.bfloat16, torch.float16)
 _bound = None
