@@ -123,6 +123,21 @@ void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
       hipLaunchKernelGGL((k_attend_join<T, 1>), joins, block, 0, s, a, p.rows, p.tile);
   }
 }
+
+template <typename T, int W>
+void verify_waves(const VerifyArgs& a, hipStream_t s) {
+  if (a.draft)
+    hipLaunchKernelGGL((k_verify<T, true, W>), dim3((unsigned)a.B), dim3(64 * W), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_verify<T, false, W>), dim3((unsigned)a.B), dim3(64 * W), 0, s, a);
+}
+template <typename T>
+void verify_launch(const VerifyArgs& a, hipStream_t s) {
+  if (a.V <= VER_SMALL)
+    verify_waves<T, 4>(a, s);
+  else
+    verify_waves<T, 16>(a, s);
+}
 }  // namespace
 
 extern "C" {
@@ -181,7 +196,7 @@ int geobpe_verify_draft(int device, void* stream, const geobpe_verify_args* p) {
   if (!p) return fail(GEOBPE_EARG, "no arguments");
   const geobpe_verify_args& x = *p;
   if (x.seqs < 0 || x.seqs > INT32_MAX || x.nodes < 1 || x.nodes > DRAFT_MAX_NODES || x.vocab < 1 ||
-      x.vocab > (int64_t)VER_TILES * VER_BLOCK * 4 || x.classes < 0 || x.classes > INT32_MAX || x.dtype < 0 || x.dtype > 2)
+      x.vocab > VER_MAX_VOCAB || x.classes < 0 || x.classes > INT32_MAX || x.dtype < 0 || x.dtype > 2)
     return fail(GEOBPE_EARG, "verify: sizes out of range");
   if (x.seqs == 0) return GEOBPE_OK;
   if (!x.d_parents || !x.d_ids || !x.d_target || !x.d_u || !x.d_n || !x.d_path || !x.d_tokens ||
@@ -196,22 +211,13 @@ int geobpe_verify_draft(int device, void* stream, const geobpe_verify_args* p) {
   a.B = (int)x.seqs, a.N = (int)x.nodes, a.V = (int)x.vocab, a.C = (int)x.classes, a.ids64 = x.ids_int64 != 0;
   OnDevice on(device);
   if (!on.ok) return fail(GEOBPE_EHIP, "verify: device %d", device);
-  const dim3 grid((unsigned)a.B), block(VER_BLOCK);
   const hipStream_t s = (hipStream_t)stream;
-#define VERIFY(T)                                                        \
-  do {                                                                   \
-    if (a.draft)                                                         \
-      hipLaunchKernelGGL((k_verify<T, true>), grid, block, 0, s, a);     \
-    else                                                                 \
-      hipLaunchKernelGGL((k_verify<T, false>), grid, block, 0, s, a);    \
-  } while (0)
   if (x.dtype == 0)
-    VERIFY(bf16_t);
+    verify_launch<bf16_t>(a, s);
   else if (x.dtype == 1)
-    VERIFY(fp16_t);
+    verify_launch<fp16_t>(a, s);
   else
-    VERIFY(float);
-#undef VERIFY
+    verify_launch<float>(a, s);
   return launched("verify");
 }
 

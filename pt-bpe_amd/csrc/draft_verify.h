@@ -10,6 +10,11 @@
 // Without draft rows q_c is one at the drafted id: r loses that entry.  Probabilities are read
 // as they are (finite positive entries, others 0); sums, products and comparisons are in 64 bits,
 // so an id near a border of two of them does not hang on the order of the sums.
+//
+// What has to be read: an entry of p and q for every node, and the rows of the contexts that a sum is needed of: the
+// last one's for the next id, others' only between a rejected child and its next sibling.  r is worked out anew from the
+// rows and the Z so far whenever it is needed, never stored.  One workgroup does a sequence: a row of 128 k entries takes
+// it about as long as the rows' share of the card's bandwidth once there are 100 sequences.
 #pragma once
 
 #include "draft.h"
@@ -29,8 +34,11 @@ struct VerifyArgs {
   int32_t ids64;
 };
 
-constexpr int VER_BLOCK = 1024;
-constexpr int VER_TILES = 1024;  // tile sums in LDS
+constexpr int VER_MAX_VOCAB = 1 << 22;
+#ifndef VER_SMALL
+#define VER_SMALL 8192
+#endif
+constexpr double VER_KEEP = 1.0 / (1 << 20);
 
 // 16 bytes of a row that is aligned to its elements only
 template <typename T>
@@ -39,83 +47,114 @@ struct alignas(sizeof(T)) VerVec {
 };
 
 template <typename T>
-__device__ inline double prob(T v) {
+__device__ inline float prob(T v) {
   const float f = (float)v;
-  return f > 0.f && f < INFINITY ? (double)f : 0.0;
+  return f > 0.f && f < INFINITY ? f : 0.f;
 }
 
-// sum over the block; every thread gets it.  red: 17 doubles of LDS.
-__device__ inline double block_sum(double v, double* red) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = v;
-  __syncthreads();
-  if (threadIdx.x < 64) {
-    double s = threadIdx.x < VER_BLOCK / 64 ? red[threadIdx.x] : 0.0;
-    for (int o = 8; o; o >>= 1) s += __shfl_xor(s, o);
-    if (threadIdx.x == 0) red[16] = s;
-  }
-  __syncthreads();
-  return red[16];
-}
-
-template <typename T>
+// a context's row with what its rejected children took
+template <typename T, bool Q>
 struct VerRow {
+  static constexpr int VEC = 16 / sizeof(T);
   const T *p, *q;
   int lo, hi;       // entries outside are 0
-  int rejected;     // siblings rejected so far
+  int rejected;     // children rejected so far
   const double* Z;  // their Z (LDS)
   const int* x;     // their ids (LDS)
 
-  // r at the VEC entries from i on (0 past hi)
-  template <bool Q>
-  __device__ void load(int i, double* r) const {
-    constexpr int VEC = 16 / sizeof(T);
-    VerVec<T> vp, vq;
-    if (i + VEC <= hi) {
-      vp = *(const VerVec<T>*)(p + i);
-      if (Q && rejected) vq = *(const VerVec<T>*)(q + i);
+  struct Raw {
+    VerVec<T> p, q;
+  };
+  __device__ bool two() const { return Q && rejected; }
+  // the VEC entries from i on (0 past end)
+  __device__ void load(Raw& w, int i, int end) const {
+    if (i + VEC <= end) {
+      w.p = *(const VerVec<T>*)(p + i);
+      if (two()) w.q = *(const VerVec<T>*)(q + i);
     } else {
+#pragma unroll
       for (int k = 0; k < VEC; k++) {
-        vp.v[k] = i + k < hi ? p[i + k] : (T)0.f;
-        vq.v[k] = Q && rejected && i + k < hi ? q[i + k] : (T)0.f;
+        w.p.v[k] = i + k < end ? p[i + k] : (T)0.f;
+        if (two()) w.q.v[k] = i + k < end ? q[i + k] : (T)0.f;
       }
     }
-    for (int k = 0; k < VEC; k++) {
-      double v = prob(vp.v[k]);
-      if (Q) {
-        if (rejected) {
-          const double w = prob(vq.v[k]);
-          for (int j = 0; j < rejected; j++) v = fmax(v - Z[j] * w, 0.0);
-        }
-      } else {
-        for (int j = 0; j < rejected; j++)
-          if (x[j] == i + k) v = 0.0;
+  }
+  __device__ void values(const Raw& w, int i, double* r) const {
+#pragma unroll
+    for (int k = 0; k < VEC; k++) r[k] = prob(w.p.v[k]);
+    if (Q) {
+      for (int j = 0; j < rejected; j++) {
+        const double z = Z[j];
+#pragma unroll
+        for (int k = 0; k < VEC; k++) r[k] = fmax(r[k] - z * (double)prob(w.q.v[k]), 0.0);
       }
-      r[k] = v;
+    } else {
+      for (int j = 0; j < rejected; j++)
+        if ((uint32_t)(x[j] - i) < (uint32_t)VEC)
+#pragma unroll
+          for (int k = 0; k < VEC; k++)
+            if (x[j] == i + k) r[k] = 0.0;
     }
+  }
+  __device__ double sum(const Raw& w, int i) const {
+    double r[VEC], s = 0;
+    values(w, i, r);
+#pragma unroll
+    for (int k = 0; k < VEC; k++) s += r[k];
+    return s;
   }
 };
 
-// One workgroup per sequence.
-template <typename T, bool Q>
-__global__ __launch_bounds__(VER_BLOCK) void k_verify(VerifyArgs a) {
-  constexpr int VEC = 16 / sizeof(T), TILE = VER_BLOCK * VEC;
-  __shared__ int par[DRAFT_MAX_NODES], depth[DRAFT_MAX_NODES], rejx[DRAFT_MAX_NODES], id[DRAFT_MAX_NODES];
-  __shared__ float u[DRAFT_MAX_NODES];
-  __shared__ double P[DRAFT_MAX_NODES], Qx[DRAFT_MAX_NODES], Z[DRAFT_MAX_NODES + 1], red[17], tile[VER_TILES];
-  __shared__ int next_;
-  const int t = threadIdx.x, b = blockIdx.x, N = a.N;
+__device__ inline double wave_total(double v) {
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// a value of one lane (the same for the whole wave)
+__device__ inline float lane_value(float v, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l)); }
+
+// One workgroup of W waves per sequence.  Every wave holds the whole tree (nodes lane and lane + 64) and makes the same
+// walk; they part only over the rows.
+template <typename T, bool Q, int W>
+__global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
+  typedef VerRow<T, Q> Row;
+  constexpr int VEC = Row::VEC, STEP = 64 * VEC, DEEP = 16 / VEC;  // (DEEP steps in flight: 128 registers hold them)
+  __shared__ double Z[DRAFT_MAX_NODES], part[W];
+  __shared__ int rejx[DRAFT_MAX_NODES];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b = blockIdx.x, N = a.N;
   const T* target = (const T*)a.target + b * a.ts[0];
   const T* draft = (const T*)a.draft + b * a.ds[0];
   const int start = a.C ? a.start[b] : 0;
-  if (t < N) {
-    par[t] = a.parents[b * a.parents_stride + t];
-    const int64_t x = a.ids64 ? ((const int64_t*)a.ids)[b * a.ids_stride + t] : ((const int32_t*)a.ids)[b * a.ids_stride + t];
-    id[t] = x < 0 || x >= a.V ? -1 : (int)x;
-    u[t] = a.u[b * a.u_stride + t];
+
+  int par[2], id[2], up[2], depth[2];
+  float u[2], P[2] = {0.f, 0.f}, q[2];
+  for (int k = 0; k < 2; k++) {
+    const int i = lane + 64 * k;
+    par[k] = -2, id[k] = -1, u[k] = 0.f, q[k] = Q ? 0.f : 1.f;
+    if (i < N) {
+      par[k] = a.parents[b * a.parents_stride + i];
+      const int64_t x =
+          a.ids64 ? ((const int64_t*)a.ids)[b * a.ids_stride + i] : ((const int32_t*)a.ids)[b * a.ids_stride + i];
+      id[k] = x < 0 || x >= a.V ? -1 : (int)x;
+      u[k] = a.u[b * a.u_stride + i];
+    }
+    // up: a node on the way to the root, depth steps above; -1: none leads there
+    up[k] = i == 0 ? (par[k] == -1 ? 0 : -1) : (par[k] >= 0 && par[k] < i ? par[k] : -1);
+    depth[k] = i > 0;
   }
-  __syncthreads();
+  auto of = [&](const int* v, int i) {  // node i's value, i of each lane's own
+    const int x = __shfl(v[0], i & 63), y = N > 64 ? __shfl(v[1], i & 63) : 0;
+    return i < 64 ? x : y;
+  };
+  while (__any(up[0] > 0 || up[1] > 0)) {  // twice the way each time
+    int nu[2], nd[2];
+    for (int k = 0; k < 2; k++) nu[k] = of(up, max(up[k], 0)), nd[k] = of(depth, max(up[k], 0));
+    for (int k = 0; k < 2; k++)
+      if (up[k] > 0) {
+        depth[k] += nd[k];
+        up[k] = nu[k];
+      }
+  }
+  const bool root = __builtin_amdgcn_readfirstlane(up[0]) == 0;
   auto range = [&](int d, int& lo, int& hi) {
     lo = 0;
     hi = a.V;
@@ -125,150 +164,160 @@ __global__ __launch_bounds__(VER_BLOCK) void k_verify(VerifyArgs a) {
     lo = max(a.ranges[2 * c], 0);
     hi = min(a.ranges[2 * c + 1], a.V);
   };
-  if (t < N) {
-    const int d = draft_depth(par, t);
-    depth[t] = d;
-    double pv = 0, qv = Q ? 0 : 1;
-    if (t && d > 0 && id[t] >= 0) {
+  bool here[2];
+  for (int k = 0; k < 2; k++) {
+    here[k] = root && up[k] == 0 && lane + 64 * k < N;
+    if (here[k] && lane + 64 * k > 0 && id[k] >= 0) {
       int lo, hi;
-      range(d - 1, lo, hi);
-      if (id[t] >= lo && id[t] < hi) {
-        pv = prob(target[par[t] * a.ts[1] + id[t]]);
-        if (Q) qv = prob(draft[par[t] * a.ds[1] + id[t]]);
+      range(depth[k] - 1, lo, hi);
+      if (id[k] >= lo && id[k] < hi) {
+        P[k] = prob(target[par[k] * a.ts[1] + id[k]]);
+        if (Q) q[k] = prob(draft[par[k] * a.ds[1] + id[k]]);
       }
     }
-    P[t] = pv;
-    Qx[t] = qv;
   }
-  __syncthreads();
   int32_t* path = a.path + (int64_t)b * N;
   int32_t* tokens = a.tokens + (int64_t)b * N;
-  if (depth[0] < 0) {
+  if (!root) {
     if (t < N) path[t] = tokens[t] = -1;
     if (t == 0) a.n[b] = 0;
     return;
   }
-  VerRow<T> row;
+
+  Row row;
+  row.Z = Z;
+  row.x = rejx;
+  // the W parts of [lo, hi) and their sums of r, all of it returned; whole steps of a wave each
+  int size = 0;
+  auto sums = [&](int lo, int hi) {
+    size = hi > lo ? ((hi - lo + W - 1) / W + STEP - 1) / STEP * STEP : STEP;
+    const int end = (int)min((int64_t)hi, (int64_t)lo + (int64_t)(wave + 1) * size);
+    double s = 0;
+    for (int64_t i = (int64_t)lo + (int64_t)wave * size + lane * VEC; i < end; i += DEEP * STEP) {
+      typename Row::Raw w[DEEP];
+#pragma unroll
+      for (int k = 0; k < DEEP; k++)
+        if (i + k * STEP < end) row.load(w[k], (int)i + k * STEP, end);
+#pragma unroll
+      for (int k = 0; k < DEEP; k++)
+        if (i + k * STEP < end) s += row.sum(w[k], (int)i + k * STEP);
+    }
+    s = wave_total(s);
+    __syncthreads();
+    if (lane == 0) part[wave] = s;
+    __syncthreads();
+    double all = lane < W ? part[lane] : 0.0;
+    return wave_total(all);
+  };
+
   int c = 0, n = 1;
-  auto context = [&](int node) {
-    c = node;
-    row.p = target + node * a.ts[1];
-    row.q = draft + node * a.ds[1];
+  if (t == 0) path[0] = 0;
+  for (;;) {
+    row.p = target + c * a.ts[1];
+    row.q = draft + c * a.ds[1];
     range(n - 1, row.lo, row.hi);
     row.rejected = 0;
-    row.Z = Z;
-    row.x = rejx;
-  };
-  // the tiles' sums of r into tile[], all of it returned
-  auto sum_row = [&]() {
-    const int tiles = row.hi > row.lo ? (row.hi - row.lo + TILE - 1) / TILE : 0;
-    for (int k = 0; k < tiles; k++) {
-      double r[VEC], s = 0;
-      const int i = row.lo + k * TILE + t * VEC;
-      row.template load<Q>(i, r);
-      for (int j = 0; j < VEC; j++) s += r[j];
-      s = block_sum(s, red);
-      if (t == 0) tile[k] = s;
-    }
-    __syncthreads();
-    double s = 0;
-    for (int k = 0; k < tiles; k++) s += tile[k];
-    return s;
-  };
-  if (t == 0) {
-    path[0] = 0;
-    Z[0] = 1.0;
-  }
-  context(0);
-  __syncthreads();
-  for (int i = 1; i < N; i++) {
-    if (depth[i] < 0 || par[i] != c) continue;
-    double r = P[i];
-    for (int j = 0; j < row.rejected; j++)
-      r = Q ? fmax(r - Z[j] * Qx[i], 0.0) : (rejx[j] == id[i] ? 0.0 : r);
-    if ((double)u[i] * Qx[i] * Z[row.rejected] < r) {
-      if (t == 0) {
-        path[n] = i;
-        tokens[n - 1] = id[i];
+    double z = 1.0, full = 0;  // Z (-1: to be taken); without draft rows the last one that was taken
+    uint64_t kids[2] = {__ballot(here[0] && par[0] == c && lane > 0), __ballot(here[1] && par[1] == c)};
+    int taken = -1;
+    uint64_t gone[2] = {0, 0};
+    while (kids[0] | kids[1]) {
+      const int k = kids[0] ? 0 : 1, l = __builtin_ctzll(kids[k]);
+      kids[k] &= kids[k] - 1;
+      const int x = __builtin_amdgcn_readlane(k ? id[1] : id[0], l);
+      const double qx = lane_value(k ? q[1] : q[0], l), ux = lane_value(k ? u[1] : u[0], l);
+      double r = lane_value(k ? P[1] : P[0], l);
+      if (row.rejected) {
+        if (z < 0) z = full = sums(row.lo, row.hi);
+        if (Q) {
+          for (int j = 0; j < row.rejected; j++) r = fmax(r - Z[j] * qx, 0.0);
+        } else {
+          if (__ballot((gone[0] >> lane & 1) && id[0] == x) | __ballot((gone[1] >> lane & 1) && id[1] == x)) r = 0;
+        }
       }
-      n++;
-      context(i);
-    } else {
-      __syncthreads();  // (others may still read the last context's rejected ids)
-      if (t == 0) rejx[row.rejected] = id[i];
+      if (ux * qx * z < r) {
+        taken = l + 64 * k;
+        if (t == 0) {
+          path[n] = taken;
+          tokens[n - 1] = x;
+        }
+        break;
+      }
+      // (every wave writes the same, and no wave is in another context while one reads: both read in sums)
+      if (Q) {
+        Z[row.rejected] = z;
+        z = -1.0;
+      } else {
+        // without draft rows the sum falls by r(x): taken anew only when little is left of it
+        gone[k] |= 1ull << l;
+        rejx[row.rejected] = x;
+        z = full > 0 && z - r > VER_KEEP * full ? z - r : -1.0;
+      }
       row.rejected++;
-      __syncthreads();
-      const double s = sum_row();
-      if (t == 0) Z[row.rejected] = s;
-      __syncthreads();
     }
+    if (taken < 0) break;
+    c = taken;
+    n++;
   }
-  double s = sum_row();
-  if (!(s > 0)) {
+  double S = sums(row.lo, row.hi);
+  if (!(S > 0)) {
     row.rejected = 0;
-    s = sum_row();
+    S = sums(row.lo, row.hi);
   }
-  // the tile, then the entry
-  const double at = (double)u[0] * s;
-  const int tiles = row.hi > row.lo ? (row.hi - row.lo + TILE - 1) / TILE : 0;
-  if (t == 0) next_ = -1;
-  double before = 0;
-  int k = 0;
-  if (s > 0) {
-    int last = 0;
-    for (int j = 0; j < tiles; j++)
-      if (tile[j] > 0) last = j;
-    for (; k < last; k++) {
-      if (before + tile[k] > at) break;
-      before += tile[k];
-    }
-    double r[VEC], mine = 0;
-    const int i = row.lo + k * TILE + t * VEC;
-    row.template load<Q>(i, r);
-    for (int j = 0; j < VEC; j++) mine += r[j];
-    // inclusive scan over the block: within the waves, then the waves' totals
-    double inc = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(inc, o);
-      if (t % 64 >= o) inc += y;
-    }
-    __syncthreads();
-    if (t % 64 == 63) red[t / 64] = inc;
-    __syncthreads();
-    double base = before;
-    for (int w = 0; w < t / 64; w++) base += red[w];
-    base += inc - mine;
-    // the first entry whose sum passes; where rounding lets none pass, the tile's last entry with mass
-    int first = INT32_MAX, lastx = -1;
-    for (int j = 0; j < VEC; j++) {
-      base += r[j];
-      if (r[j] > 0) {
-        lastx = i + j;
-        if (base > at && first == INT32_MAX) first = i + j;
+  // the part that the number falls into, a part of it, and so on down to a few steps of one wave
+  int next = -1;
+  if (S > 0) {
+    double at = (double)lane_value(u[0], 0) * S;
+    int lo = row.lo, hi = row.hi;
+    for (;;) {
+      double in = lane < W ? part[lane] : 0.0;
+      const uint64_t some = __ballot(in > 0);
+      const double mine = in;
+      for (int o = 1; o < W; o <<= 1) {
+        const double y = __shfl_up(in, o);
+        if (lane >= o) in += y;
       }
+      const uint64_t over = __ballot(lane < W && mine > 0 && in > at);
+      const int w = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);  // (rounding let none pass: the last)
+      at -= __shfl(in - mine, w);
+      lo += w * size;
+      hi = (int)min((int64_t)hi, (int64_t)lo + size);
+      if (hi - lo <= DEEP * STEP) break;
+      sums(lo, hi);
     }
-    for (int o = 32; o; o >>= 1) {
-      first = min(first, __shfl_xor(first, o));
-      lastx = max(lastx, __shfl_xor(lastx, o));
-    }
-    int* fl = (int*)tile;  // (the tile sums are done with)
-    __syncthreads();
-    if (t % 64 == 0) {
-      fl[t / 64] = first;
-      fl[16 + t / 64] = lastx;
-    }
-    __syncthreads();
-    if (t == 0) {
-      for (int w = 1; w < 16; w++) {
-        first = min(first, fl[w]);
-        lastx = max(lastx, fl[16 + w]);
+    int last = -1;
+    for (int i = lo; i < hi && next < 0; i += STEP) {
+      typename Row::Raw w;
+      double r[VEC], mine = 0;
+      const int e = i + lane * VEC;
+      row.load(w, e, hi);
+      row.values(w, e, r);
+#pragma unroll
+      for (int k = 0; k < VEC; k++) mine += r[k];
+      double in = mine;
+      for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(in, o);
+        if (lane >= o) in += y;
       }
-      next_ = first != INT32_MAX ? first : lastx;
+      double base = in - mine;
+      int first = INT32_MAX, back = -1;
+#pragma unroll
+      for (int k = 0; k < VEC; k++) {
+        base += r[k];
+        if (r[k] > 0) {
+          back = e + k;
+          if (base > at && first == INT32_MAX) first = e + k;
+        }
+      }
+      const uint64_t hit = __ballot(first != INT32_MAX), some = __ballot(back >= 0);
+      if (hit) next = __shfl(first, __builtin_ctzll(hit));
+      if (some) last = __shfl(back, 63 - __builtin_clzll(some));
+      at -= __shfl(in, 63);
     }
+    if (next < 0) next = last;
   }
-  __syncthreads();
   if (t == 0) {
-    tokens[n - 1] = next_;
+    tokens[n - 1] = next;
     a.n[b] = n;
   }
   if (t >= n && t < N) path[t] = tokens[t] = -1;
