@@ -49,7 +49,7 @@ struct alignas(sizeof(T)) VerVec {
 template <typename T>
 __device__ inline float prob(T v) {
   const float f = (float)v;
-  return f > 0.f && f < INFINITY ? f : 0.f;
+  return __builtin_amdgcn_classf(f, 0x180) ? f : 0.f;  // positive, finite
 }
 
 // a context's row with what its rejected children took
@@ -105,10 +105,30 @@ struct VerRow {
   }
 };
 
-__device__ inline double wave_total(double v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+// v of the lane CTRL says (0 where it says none), for the lanes of the rows in MASK
+template <int CTRL, int MASK>
+__device__ inline double dpp(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, MASK, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, MASK, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// sums over the lanes up to each (rows of 16 lanes first, then the rows before), without LDS
+__device__ inline double wave_scan(double v) {
+  v += dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+  v += dpp<0x112, 0xf>(v);
+  v += dpp<0x114, 0xf>(v);
+  v += dpp<0x118, 0xf>(v);
+  v += dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
+__device__ inline double lane_value(double v, int l) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)u, l), hi = __builtin_amdgcn_readlane((int)(u >> 32), l);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ inline double wave_total(double v) { return lane_value(wave_scan(v), 63); }
 // a value of one lane (the same for the whole wave)
 __device__ inline float lane_value(float v, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l)); }
 
@@ -117,9 +137,10 @@ __device__ inline float lane_value(float v, int l) { return __uint_as_float(__bu
 template <typename T, bool Q, int W>
 __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
   typedef VerRow<T, Q> Row;
-  constexpr int VEC = Row::VEC, STEP = 64 * VEC, DEEP = 16 / VEC;  // (DEEP steps in flight: 128 registers hold them)
+  constexpr int VEC = Row::VEC, STEP = 64 * VEC, DEEP = (Q && W > 4 ? 16 : 32) / VEC;  // steps in flight (with 16 waves 128 registers have to hold them)
   __shared__ double Z[DRAFT_MAX_NODES], part[W];
   __shared__ int rejx[DRAFT_MAX_NODES];
+  __shared__ double rejr[Q ? 1 : DRAFT_MAX_NODES];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b = blockIdx.x, N = a.N;
   const T* target = (const T*)a.target + b * a.ts[0];
   const T* draft = (const T*)a.draft + b * a.ds[0];
@@ -210,14 +231,17 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
     return wave_total(all);
   };
 
-  int c = 0, n = 1;
+  int c = 0, n = 1, seen = 0;
+  double z = 1.0, full = 0;
   if (t == 0) path[0] = 0;
   for (;;) {
     row.p = target + c * a.ts[1];
     row.q = draft + c * a.ds[1];
     range(n - 1, row.lo, row.hi);
     row.rejected = 0;
-    double z = 1.0, full = 0;  // Z (-1: to be taken); without draft rows the last one that was taken
+    z = 1.0;    // Z (-1: to be taken)
+    full = 0;   // without draft rows the last one that was taken,
+    seen = 0;   // and the children rejected by then
     uint64_t kids[2] = {__ballot(here[0] && par[0] == c && lane > 0), __ballot(here[1] && par[1] == c)};
     int taken = -1;
     uint64_t gone[2] = {0, 0};
@@ -228,7 +252,10 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
       const double qx = lane_value(k ? q[1] : q[0], l), ux = lane_value(k ? u[1] : u[0], l);
       double r = lane_value(k ? P[1] : P[0], l);
       if (row.rejected) {
-        if (z < 0) z = full = sums(row.lo, row.hi);
+        if (z < 0) {
+          z = full = sums(row.lo, row.hi);
+          seen = row.rejected;
+        }
         if (Q) {
           for (int j = 0; j < row.rejected; j++) r = fmax(r - Z[j] * qx, 0.0);
         } else {
@@ -251,6 +278,7 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
         // without draft rows the sum falls by r(x): taken anew only when little is left of it
         gone[k] |= 1ull << l;
         rejx[row.rejected] = x;
+        rejr[row.rejected] = r;
         z = full > 0 && z - r > VER_KEEP * full ? z - r : -1.0;
       }
       row.rejected++;
@@ -259,7 +287,21 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
     c = taken;
     n++;
   }
-  double S = sums(row.lo, row.hi);
+  double S = -1.0;
+  if (!Q && full > 0 && row.rejected > seen) {
+    // the parts are known from the last sum, but for the entries that went since: taken off, unless a part loses nearly all
+    double mine = lane < W ? part[lane] : 0.0;
+    const double before = mine;
+    for (int j = seen; j < row.rejected; j++)
+      if (lane == (rejx[j] - row.lo) / size) mine -= rejr[j];
+    if (!__any(mine < before && !(mine > VER_KEEP * before))) {
+      __syncthreads();
+      if (wave == 0 && lane < W) part[lane] = mine;
+      __syncthreads();
+      S = wave_total(mine);
+    }
+  }
+  if (S < 0) S = sums(row.lo, row.hi);
   if (!(S > 0)) {
     row.rejected = 0;
     S = sums(row.lo, row.hi);
@@ -270,35 +312,30 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
     double at = (double)lane_value(u[0], 0) * S;
     int lo = row.lo, hi = row.hi;
     for (;;) {
-      double in = lane < W ? part[lane] : 0.0;
-      const uint64_t some = __ballot(in > 0);
-      const double mine = in;
-      for (int o = 1; o < W; o <<= 1) {
-        const double y = __shfl_up(in, o);
-        if (lane >= o) in += y;
-      }
+      const double mine = lane < W ? part[lane] : 0.0, in = wave_scan(mine);
+      const uint64_t some = __ballot(mine > 0);
       const uint64_t over = __ballot(lane < W && mine > 0 && in > at);
       const int w = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);  // (rounding let none pass: the last)
-      at -= __shfl(in - mine, w);
+      at -= lane_value(in - mine, w);
       lo += w * size;
       hi = (int)min((int64_t)hi, (int64_t)lo + size);
       if (hi - lo <= DEEP * STEP) break;
       sums(lo, hi);
     }
     int last = -1;
-    for (int i = lo; i < hi && next < 0; i += STEP) {
-      typename Row::Raw w;
+    typename Row::Raw w[DEEP];
+#pragma unroll
+    for (int k = 0; k < DEEP; k++)
+      if (lo + k * STEP < hi) row.load(w[k], lo + k * STEP + lane * VEC, hi);
+#pragma unroll
+    for (int j = 0; j < DEEP; j++) {
+      if (lo + j * STEP >= hi || next >= 0) break;
       double r[VEC], mine = 0;
-      const int e = i + lane * VEC;
-      row.load(w, e, hi);
-      row.values(w, e, r);
+      const int e = lo + j * STEP + lane * VEC;
+      row.values(w[j], e, r);
 #pragma unroll
       for (int k = 0; k < VEC; k++) mine += r[k];
-      double in = mine;
-      for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(in, o);
-        if (lane >= o) in += y;
-      }
+      const double in = wave_scan(mine);
       double base = in - mine;
       int first = INT32_MAX, back = -1;
 #pragma unroll
@@ -310,9 +347,9 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
         }
       }
       const uint64_t hit = __ballot(first != INT32_MAX), some = __ballot(back >= 0);
-      if (hit) next = __shfl(first, __builtin_ctzll(hit));
-      if (some) last = __shfl(back, 63 - __builtin_clzll(some));
-      at -= __shfl(in, 63);
+      if (hit) next = __builtin_amdgcn_readlane(first, __builtin_ctzll(hit));
+      if (some) last = __builtin_amdgcn_readlane(back, 63 - __builtin_clzll(some));
+      at -= lane_value(in, 63);
     }
     if (next < 0) next = last;
   }
