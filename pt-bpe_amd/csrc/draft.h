@@ -13,17 +13,19 @@ namespace gb {
 constexpr int DRAFT_MAX_NODES = 128;
 constexpr int DRAFT_MAX_POSITIONS = 0x7ffff000;  // a sequence's; some tiles of keys more stay an int32
 
-// depth of node i (root: 0), -1 when it is absent.  par: the tree's parents (N of them, LDS).
-// Every step goes to a smaller index, so the walk ends within i steps.
-__device__ inline int draft_depth(const int* par, int i) {
-  int d = 0;
-  while (i > 0) {
+// the nodes on the path from the root to i as bits of w (i included); false, and w empty, when i is absent.
+// par: the tree's parents.  Every step goes to a smaller index, so the walk ends within i steps.
+__device__ inline bool draft_path(const int* par, int i, uint32_t w[DRAFT_MAX_NODES / 32]) {
+  for (int k = 0; k < DRAFT_MAX_NODES / 32; k++) w[k] = 0;
+  for (;;) {
+    for (int k = 0; k < DRAFT_MAX_NODES / 32; k++) w[k] |= i / 32 == k ? 1u << (i % 32) : 0u;
     const int p = par[i];
-    if (p < 0 || p >= i) return -1;
+    if (p < 0 || p >= i) break;
     i = p;
-    d++;
   }
-  return par[0] == -1 ? d : -1;
+  const bool here = i == 0 && par[0] == -1;
+  for (int k = 0; k < DRAFT_MAX_NODES / 32; k++) w[k] = here ? w[k] : 0u;
+  return here;
 }
 
 // x / d for 0 <= x < 2^31 and 1 <= d < 2^31, with the host's m = min(2^32 / d, 2^32 - 1) rounded down: x m / 2^32

@@ -50,23 +50,32 @@ bool aligned(const void* p, const int64_t* strides, int n, int64_t unit) {
 }
 
 // how a call is cut: rows a workgroup works on, tiles of keys a part has at most
+#ifndef WANT_S
+#define WANT_S 1024
+#endif
 struct AttendPlan {
-  bool wide;
-  int rb, rows, tile, per, most;
+  bool wide, sorted;
+  int rb, waves, rows, tile, per, most;
   int64_t row_tiles, blocks, bytes;
 };
 AttendPlan attend_plan(const geobpe_attend_args& x) {
   AttendPlan p;
   const int64_t M = x.nodes * (x.heads / x.kv_heads);
-  p.wide = M > 32;
+  p.wide = M > (x.head_dim > 128 ? 16 : 32);
   p.rb = M <= 16 ? 1 : 2;
   p.rows = p.wide ? WIDE_ROWS : 16 * p.rb;
   p.tile = p.wide ? WIDE_TILE : ATT_TILE;
   p.row_tiles = (M + p.rows - 1) / p.rows;
   const int64_t tiles = (x.max_pages * x.page_size + p.tile - 1) / p.tile + (x.nodes + p.tile - 1) / p.tile;
-  const int64_t items = x.seqs * x.kv_heads, even = (items * p.row_tiles * tiles + ATT_WANT - 1) / ATT_WANT;
+  const int64_t items = x.seqs * x.kv_heads;
+  // eight waves where that fills the card without cutting the sequences (64 sequences x 4 heads: 26 us instead of 25 + 10
+  // for the join); four where they are cut anyway, and more finely then (7 x 12 heads: 27 us instead of 40)
+  p.waves = !p.wide && x.head_dim <= 128 && items * p.row_tiles >= 128 && items * p.row_tiles <= 256 ? 8 : 4;
+  p.sorted = p.wide && x.seqs > 1 && x.seqs <= ATT_SORT;
+  const int64_t want = p.waves == 8 ? ATT_WANT / 2 : p.sorted ? WANT_S : ATT_WANT, even = (items * p.row_tiles * tiles + want - 1) / want;
   p.per = (int)(even > tiles ? tiles : even > ATT_LEAST ? even : ATT_LEAST);
   p.most = (int)((tiles + p.per - 1) / p.per);
+  p.sorted = p.sorted && items * p.most * p.row_tiles > 512;
   p.blocks = (items * p.most + 7) / 8 * 8 * p.row_tiles;
   p.bytes = p.most > 1 ? items * p.row_tiles * p.most * p.rows * (x.head_dim + 2) * 4 : 0;
   return p;
@@ -87,35 +96,50 @@ int attend_sizes(const geobpe_attend_args& x) {
 
 template <typename T, int KS>
 void attend_narrow(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.blocks), block(ATT_BLOCK);
-  if (p.rb == 1)
-    hipLaunchKernelGGL((k_attend<T, KS, 1>), grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL((k_attend<T, KS, 2>), grid, block, 0, s, a);
+  const dim3 grid((unsigned)p.blocks), block(64 * p.waves);
+  if constexpr (KS > 4) {
+    hipLaunchKernelGGL((k_attend<T, KS, 1, 4>), grid, block, 0, s, a);
+  } else if (p.waves == 8) {
+    if (p.rb == 1)
+      hipLaunchKernelGGL((k_attend<T, KS, 1, 8>), grid, block, 0, s, a);
+    else
+      hipLaunchKernelGGL((k_attend<T, KS, 2, 8>), grid, block, 0, s, a);
+  } else {
+    if (p.rb == 1)
+      hipLaunchKernelGGL((k_attend<T, KS, 1, 4>), grid, block, 0, s, a);
+    else
+      hipLaunchKernelGGL((k_attend<T, KS, 2, 4>), grid, block, 0, s, a);
+  }
 }
 template <typename T>
 void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)p.blocks), block(ATT_BLOCK);
   if (p.wide) {
-    if (a.D <= 64)
-      hipLaunchKernelGGL((k_attend_wide<T, 64>), grid, block, 0, s, a);
-    else if (a.D <= 128)
-      hipLaunchKernelGGL((k_attend_wide<T, 128>), grid, block, 0, s, a);
+    if (a.D == 64)
+      hipLaunchKernelGGL((k_attend_wide<T, 64, true>), grid, block, 0, s, a);
+    else if (a.D < 64)
+      hipLaunchKernelGGL((k_attend_wide<T, 64, false>), grid, block, 0, s, a);
+    else if (a.D == 128)
+      hipLaunchKernelGGL((k_attend_wide<T, 128, true>), grid, block, 0, s, a);
+    else if (a.D < 128)
+      hipLaunchKernelGGL((k_attend_wide<T, 128, false>), grid, block, 0, s, a);
     else
-      hipLaunchKernelGGL((k_attend_wide<T, 256>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((k_attend_wide<T, 256, false>), grid, block, 0, s, a);
   } else {
     switch ((a.D + 31) / 32) {
       case 1: attend_narrow<T, 1>(a, p, s); break;
       case 2: attend_narrow<T, 2>(a, p, s); break;
       case 3: attend_narrow<T, 3>(a, p, s); break;
       case 4: attend_narrow<T, 4>(a, p, s); break;
+      case 5:
+      case 6: attend_narrow<T, 6>(a, p, s); break;
       default: attend_narrow<T, 8>(a, p, s);
     }
   }
   if (p.most > 1) {
-    // eight threads over a row's parts where there are too few rows to fill the card
+    // eight threads over a row's parts where they are many and the rows too few to fill the card
     const int64_t rows = (int64_t)a.B * a.N * a.Hq;
-    const int by = rows * (a.D / 4) < 512 * ATT_BLOCK && a.D <= 128 ? 8 : 1, each = ATT_BLOCK / (a.D / 4 * by);
+    const int by = p.most > 16 && rows * (a.D / 4) < 512 * ATT_BLOCK && a.D <= 128 ? 8 : 1, each = ATT_BLOCK / (a.D / 4 * by);
     const dim3 joins((unsigned)((rows + each - 1) / each));
     if (by == 8)
       hipLaunchKernelGGL((k_attend_join<T, 8>), joins, block, 0, s, a, p.rows, p.tile);
@@ -182,6 +206,7 @@ int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p,
   a.scale = (float)x.scale;
   a.per = plan.per;
   a.most = plan.most;
+  a.sorted = plan.sorted;
   a.part = (float*)d_work;
   OnDevice on(device);
   if (!on.ok) return fail(GEOBPE_EHIP, "tree attention: device %d", device);

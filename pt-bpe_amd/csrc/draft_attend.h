@@ -25,6 +25,7 @@ struct AttendArgs {
   PageDiv div;
   float scale;
   int32_t per, most;  // tiles a part of a sequence's keys has at most, parts there are room for
+  int32_t sorted;     // long parts first
   float* part;        // [row tile][item][part][row][D], then {max, sum} [row tile][item][part][row]
 };
 
@@ -34,7 +35,15 @@ constexpr int ATT_TILE = 32;  // keys a wave works on at a time
 // The keys are cut so that about two workgroups a CU have work (more parts cost their joining: at 512 / 1024 / 2048
 // workgroups 64 trees of 5 nodes over up to 2237 positions took 42 / 49 / 44 us, 32 of 64 nodes over up to 16 k 610 /
 // 631 / 656), but no part gets below 16 tiles (with 8 one token over 237 positions took 10.8 us instead of 8.2).
-constexpr int ATT_WANT = 512, ATT_LEAST = 16;
+#ifndef NSETS
+#define NSETS 1
+#endif
+#ifndef WANT
+#define WANT 512
+#define LEAST 16
+#endif
+constexpr int ATT_WANT = WANT, ATT_LEAST = LEAST;
+constexpr int ATT_SORT = ATT_BLOCK;  // sequences that are sorted at most
 constexpr float LOG2E = 1.44269504088896340736f;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -123,16 +132,15 @@ struct Tree {
   int par[DRAFT_MAX_NODES];
   uint32_t anc[DRAFT_MAX_NODES][4];
 };
-__device__ inline void tree_paths(Tree& tr, int N, const int32_t* parents) {
+// in two halves, so that what the caller loads meanwhile is not waited for in between
+__device__ inline int tree_parent(int N, const int32_t* parents) { return threadIdx.x < N ? parents[threadIdx.x] : 0; }
+__device__ inline void tree_paths(Tree& tr, int N, int parent) {
   const int t = threadIdx.x;
-  if (t < N) tr.par[t] = parents[t];
+  if (t < N) tr.par[t] = parent;
   __syncthreads();
   if (t < N) {
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (draft_depth(tr.par, t) >= 0)
-      for (int i = t; i >= 0; i = tr.par[i])
-        for (int k = 0; k < 4; k++)
-          if (i / 32 == k) w[k] |= 1u << (i % 32);
+    uint32_t w[4];
+    draft_path(tr.par, t, w);
     for (int k = 0; k < 4; k++) tr.anc[t][k] = w[k];
   }
   __syncthreads();
@@ -169,6 +177,37 @@ __device__ inline Share share_of(const AttendArgs& a, int tiles, int part) {
   s.last = min(s.first + size, tiles);
   return s;
 }
+// Which part of which item a workgroup has.  Sequences of different lengths are taken in the order of their parts'
+// sizes, the largest first, so that the last workgroups to start are short ones (32 x 64 nodes over 8 to 16 k
+// positions: see k_attend_wide).  Every workgroup works that out by itself, a thread a sequence.
+struct Work {
+  int b, h, part;
+};
+__device__ inline Work work_of(const AttendArgs& a, int work, int tile) {
+  if (!a.sorted) return {uni(work / a.most / a.Hkv), uni(work / a.most % a.Hkv), uni(work % a.most)};
+  __shared__ int size[ATT_SORT], count[ATT_SORT], found[2];
+  const int t = threadIdx.x;
+  int mine = 0;
+  if (t < a.B) {
+    const int tiles = span_of(a, t, tile).tiles;
+    const Share s = share_of(a, tiles, 0);
+    size[t] = mine = s.last;
+    count[t] = s.parts * a.Hkv;
+  }
+  if (t == 0) found[0] = -1;
+  __syncthreads();
+  if (t < a.B) {
+    int before = 0;
+    for (int b = 0; b < a.B; b++)
+      if (size[b] > mine || (size[b] == mine && b < t)) before += count[b];
+    if (work >= before && work < before + count[t]) {
+      found[0] = t;
+      found[1] = work - before;
+    }
+  }
+  __syncthreads();
+  return {uni(found[0]), uni(found[1] % a.Hkv), uni(found[1] / a.Hkv)};
+}
 // a row's place among the parts
 __device__ inline int64_t part_row(const AttendArgs& a, int rt, int item, int part, int rows, int row) {
   return (((int64_t)rt * a.B * a.Hkv + item) * a.most + part) * rows + row;
@@ -185,13 +224,14 @@ __device__ inline float* part_sums(const AttendArgs& a, int RT, int rows) {
 // product's operand wants, so nothing is moved between lanes but the maximum.  K goes from memory into the operand
 // registers, V through the wave's own LDS, where the transposing read turns it; the rows there are 32 bytes longer
 // than the head so that eight of them start in different banks.
-template <typename T, int KS, int RB>
-__global__ __launch_bounds__(ATT_BLOCK, KS > 4 ? 1 : 2) void k_attend(AttendArgs a) {
+template <typename T, int KS, int RB, int W>
+__global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 : 1) void k_attend(AttendArgs a) {
   constexpr int DP = 32 * KS, DB = 2 * KS, LROW = DP * 2 + 32;
+  constexpr int DMIN = KS <= 4 ? DP - 24 : DP - 56, SETS = KS <= 4 ? NSETS : 1;  // the heads this is for: DMIN .. DP
   constexpr int AREA = ATT_TILE * LROW;  // >= 16 rows of DP + 4 floats
-  __shared__ __attribute__((aligned(16))) char lds[ATT_WAVES * AREA];
+  __shared__ __attribute__((aligned(16))) char lds[W * AREA];
   __shared__ Tree tr;
-  __shared__ float ml[2][ATT_WAVES][RB * 16];
+  __shared__ float ml[2][W][RB * 16];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l16 = lane & 15, lq = lane >> 4;
   const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + RB * 16 - 1) / (RB * 16);
   // blocks go to the 8 dies in turn: the row tiles of one part stay on one die, one after the other
@@ -212,44 +252,8 @@ __global__ __launch_bounds__(ATT_BLOCK, KS > 4 ? 1 : 2) void k_attend(AttendArgs
   const T* vd = (const T*)a.vd + b * a.vds[0] + h * a.vds[2];
   bool bad = sp.bad;
 
-  // a tile's addresses: lane's keys are l16 and 16 + l16 of it, keys past the end are the last key again.  The
-  // table's entries are looked at only when they are used, a tile later: nothing waits for them before.
-  int id[2], slot[2];
-  auto find = [&](int tile) {
-    for (int c = 0; c < 2; c++) id[c] = page_entry(pages, min(tile * ATT_TILE + 16 * c + l16, sp.len - 1), slot[c]);
-  };
-  u32x4 kf[2][KS], vf[2][KS];
-  auto load = [&](int c, const T* kp, const T* vp) {
-    for (int k = 0; k < KS; k++) {
-      const int d = 32 * k + 8 * lq;
-      const u32x4 zero = {0, 0, 0, 0};
-      kf[c][k] = d < a.D ? *(const u32x4*)(kp + d) : zero;
-      vf[c][k] = d < a.D ? *(const u32x4*)(vp + d) : zero;
-    }
-  };
-  auto fetch = [&]() {
-    for (int c = 0; c < 2; c++) {
-      if (!good_page(pages, id[c])) {  // reads page 0, and the sequence's rows become NaN
-        bad = true;
-        id[c] = 0;
-      }
-      load(c, (const T*)(kc + cache_row(id[c], slot[c], a.kpage, a.kslot)),
-           (const T*)(vc + cache_row(id[c], slot[c], a.vpage, a.vslot)));
-    }
-  };
-  auto fetch_nodes = [&](int base) {
-    for (int c = 0; c < 2; c++) {
-      const int n = min(base + 16 * c + l16, a.N - 1);
-      load(c, kd + n * a.kds[1], vd + n * a.vds[1]);
-    }
-  };
-  const int cached = min(last, sp.cache_tiles);
-  int tile = first + wave;
-  if (tile < cached) {
-    find(tile);
-    fetch();
-    if (tile + ATT_WAVES < cached) find(tile + ATT_WAVES);
-  }
+  // what does not hang on the length is loaded first
+  const int parent = tree_parent(a.N, a.parents + b * a.parents_stride);
   u32x4 qf[RB][KS];
   for (int r = 0; r < RB; r++) {
     const int m = (rt * RB + r) * 16 + l16, n = m / G;
@@ -260,7 +264,53 @@ __global__ __launch_bounds__(ATT_BLOCK, KS > 4 ? 1 : 2) void k_attend(AttendArgs
       qf[r][k] = m < M && d < a.D ? signed_by(*(const u32x4*)(q + d), a.scale) : zero;
     }
   }
-  tree_paths(tr, a.N, a.parents + b * a.parents_stride);
+  // A tile as the lane loads it: keys l4 and 16 + l4 (past the end the last key again), pieces 4 k + p4 of them, so that
+  // four lanes in a row read 64 bytes in a row (in the operands' own order, a key a lane, the L1 took three times as
+  // many accesses and the kernel 1.4 times as long).  The table's entries are looked at only when they are used, a turn
+  // later: nothing waits for them before.
+  const int l4 = lane >> 2, p4 = lane & 3;
+  struct Tile {
+    u32x4 k[2][KS], v[2][KS];
+    int id[2], slot[2];
+  };
+  auto find = [&](Tile& x, int tile) {
+    for (int c = 0; c < 2; c++)
+      x.id[c] = page_entry(pages, min(tile * ATT_TILE + 16 * c + l4, sp.len - 1), x.slot[c]);
+  };
+  auto load = [&](Tile& x, int c, const T* kp, const T* vp) {
+    for (int k = 0; k < KS; k++) {
+      const int d = 32 * k + 8 * p4;
+      if (32 * k + 32 <= DMIN) {
+        x.k[c][k] = *(const u32x4*)(kp + d);
+        x.v[c][k] = *(const u32x4*)(vp + d);
+      } else {  // (past the head: K is 0 there, as the query is; V's channels there go nowhere)
+        const bool in = d < a.D;
+        const u32x4 y = *(const u32x4*)(kp + (in ? d : 0));
+        for (int i = 0; i < 4; i++) x.k[c][k][i] = in ? y[i] : 0u;
+        x.v[c][k] = *(const u32x4*)(vp + (in ? d : 0));
+      }
+    }
+  };
+  auto fetch = [&](Tile& x) {
+    for (int c = 0; c < 2; c++) {
+      if (!good_page(pages, x.id[c])) {  // reads page 0, and the sequence's rows become NaN
+        bad = true;
+        x.id[c] = 0;
+      }
+      load(x, c, (const T*)(kc + cache_row(x.id[c], x.slot[c], a.kpage, a.kslot)),
+           (const T*)(vc + cache_row(x.id[c], x.slot[c], a.vpage, a.vslot)));
+    }
+  };
+  // SETS tiles of a wave are on their way at a time
+  const int cached = min(last, sp.cache_tiles);
+  int tile = first + wave;
+  Tile x[SETS];
+  if (tile < cached) {
+    for (int i = 0; i < SETS; i++) find(x[i], tile + i * W);
+    for (int i = 0; i < SETS; i++) fetch(x[i]);
+    for (int i = 0; i < SETS; i++) find(x[i], tile + (SETS + i) * W);
+  }
+  tree_paths(tr, a.N, parent);
 
   float top[RB], sum[RB];
   f32x4 o[DB][RB];
@@ -269,19 +319,28 @@ __global__ __launch_bounds__(ATT_BLOCK, KS > 4 ? 1 : 2) void k_attend(AttendArgs
     sum[r] = 0.f;
     for (int d = 0; d < DB; d++) o[d][r] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  auto step = [&](auto is_nodes, int base) {
+  auto step = [&](auto is_nodes, int base, Tile& x, int tile) {
     constexpr bool nodes = decltype(is_nodes)::value;
+    // K into the operands' order through the wave's LDS, then V there for the transposing read
+    char* mine = area + l4 * LROW + p4 * 16;
+    for (int c = 0; c < 2; c++)
+      for (int k = 0; k < KS; k++) *(u32x4*)(mine + c * 16 * LROW + k * 64) = x.k[c][k];
+    wave_order();
+    u32x4 kf[2][KS];
+    for (int c = 0; c < 2; c++)
+      for (int k = 0; k < KS; k++) kf[c][k] = *(const u32x4*)(area + (16 * c + l16) * LROW + k * 64 + lq * 16);
+    wave_order();
     bool odd = false;  // a node's value that is not finite
     for (int c = 0; c < 2; c++)
       for (int k = 0; k < KS; k++) {
         if constexpr (nodes) {
           // a node reaches its own descendants only, but 0 times infinity or NaN would reach every row:
           // such values go in as 0 and are added below where they belong
-          const bool bad_v = not_finite<T>(vf[c][k]);
+          const bool bad_v = not_finite<T>(x.v[c][k]);
           odd |= bad_v;
-          for (int i = 0; i < 4; i++) vf[c][k][i] = bad_v ? 0u : vf[c][k][i];
+          for (int i = 0; i < 4; i++) x.v[c][k][i] = bad_v ? 0u : x.v[c][k][i];
         }
-        *(u32x4*)(area + (16 * c + l16) * LROW + (32 * k + 8 * lq) * 2) = vf[c][k];
+        *(u32x4*)(mine + c * 16 * LROW + k * 64) = x.v[c][k];
       }
     wave_order();
     f32x4 s[2][RB];
@@ -290,10 +349,9 @@ __global__ __launch_bounds__(ATT_BLOCK, KS > 4 ? 1 : 2) void k_attend(AttendArgs
         s[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < KS; k++) s[c][r] = Half<T>::mfma(kf[c][k], qf[r][k], s[c][r]);
       }
-    const int next = tile + ATT_WAVES;
-    if (!nodes && next < cached) {
-      fetch();
-      if (next + ATT_WAVES < cached) find(next + ATT_WAVES);
+    if (!nodes && tile + SETS * W < cached) {
+      fetch(x);
+      find(x, tile + 2 * SETS * W);
     }
     u32x4 p[RB];
     for (int r = 0; r < RB; r++) {
@@ -373,11 +431,22 @@ __global__ __launch_bounds__(ATT_BLOCK, KS > 4 ? 1 : 2) void k_attend(AttendArgs
       wave_order();
     }
   };
-  for (; tile < cached; tile += ATT_WAVES) step(std::false_type(), tile * ATT_TILE);
-  for (; tile < last; tile += ATT_WAVES) {
+  while (tile < cached) {
+#pragma unroll
+    for (int i = 0; i < SETS; i++) {
+      if (tile < cached) {
+        step(std::false_type(), tile * ATT_TILE, x[i], tile);
+        tile += W;
+      }
+    }
+  }
+  for (; tile < last; tile += W) {
     const int base = (tile - sp.cache_tiles) * ATT_TILE;
-    fetch_nodes(base);
-    step(std::true_type(), base);
+    for (int c = 0; c < 2; c++) {
+      const int n = min(base + 16 * c + l4, a.N - 1);
+      load(x[0], c, kd + n * a.kds[1], vd + n * a.vds[1]);
+    }
+    step(std::true_type(), base, x[0], tile);
   }
 
   // the waves' sums joined: maxima first, then 16 rows at a time through LDS
@@ -394,15 +463,15 @@ __global__ __launch_bounds__(ATT_BLOCK, KS > 4 ? 1 : 2) void k_attend(AttendArgs
     float* mine = (float*)area + l16 * (DP + 4) + 4 * lq;
     for (int d = 0; d < DB; d++) *(f32x4*)(mine + 16 * d) = o[d][r];
     __syncthreads();
-    for (int e = t; e < 16 * DP / 4; e += ATT_BLOCK) {
+    for (int e = t; e < 16 * DP / 4; e += 64 * W) {
       const int row = e / (DP / 4), d = e % (DP / 4) * 4, m = (rt * RB + r) * 16 + row;
       if (m >= M || d >= a.D) continue;
       float mx = -INFINITY;
-      for (int w = 0; w < ATT_WAVES; w++) mx = fmaxf(mx, ml[0][w][r * 16 + row]);
+      for (int w = 0; w < W; w++) mx = fmaxf(mx, ml[0][w][r * 16 + row]);
       const float from = at_least(mx);
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       float total = 0.f;
-      for (int w = 0; w < ATT_WAVES; w++) {
+      for (int w = 0; w < W; w++) {
         const float f = __builtin_amdgcn_exp2f((ml[0][w][r * 16 + row] - from) * scale);
         total += f * ml[1][w][r * 16 + row];
         acc += f * *(const f32x4*)((const float*)(lds + w * AREA) + row * (DP + 4) + d);
@@ -482,7 +551,7 @@ __device__ inline void wait_loads() {
 
 __device__ const u32x4 att_zero = {0, 0, 0, 0};  // what a head's pieces past its end are read from
 
-template <typename T, int DP>
+template <typename T, int DP, bool FULL>
 __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(AttendArgs a) {
   constexpr int CH = DP / 8, KSTEPS = DP / 16, DB = DP / 32;
   constexpr int TILE_BYTES = WIDE_TILE * DP * 2, PER = WIDE_TILE * CH / ATT_BLOCK;  // pieces a thread moves
@@ -499,7 +568,9 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
   const int die = blockIdx.x & 7, j8 = blockIdx.x >> 3;
   const int rt = uni(j8 % RT), work = uni((j8 / RT) * 8 + die);
   if (work >= a.B * a.Hkv * a.most) return;
-  const int part = uni(work % a.most), item = uni(work / a.most), h = uni(item % a.Hkv), b = uni(item / a.Hkv);
+  const Work wk = work_of(a, work, WIDE_TILE);
+  if (wk.b < 0) return;
+  const int b = wk.b, h = wk.h, part = wk.part, item = b * a.Hkv + h;
   const Span sp = span_of(a, b, WIDE_TILE);
   const Share sh = share_of(a, sp.tiles, part);
   if (part >= sh.parts) return;
@@ -519,8 +590,8 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
   const int prow = t / CH, pc = t % CH;
 
   {
-    const int last = uni(sh.last), cached = min(last, uni(sp.cache_tiles));
-    int tile = uni(sh.first);
+    const int first = uni(sh.first), last = uni(sh.last), cached = min(last, uni(sp.cache_tiles));
+    int tile = first;
     bool bad = sp.bad;
     float top = -INFINITY, sum = 0.f;  // the row's reference and its sum of weights
     f32x16 o[DB];
@@ -572,94 +643,89 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
     {
       const int len = uni(sp.len);
       if (t == 0) odd_ = 0;
-      const Pages pages = {a.table + b * a.table_stride, a.div, a.P, a.M};
-      const char* kc = (const char*)((const T*)a.kc + h * a.khead);
-      const char* vc = (const char*)((const T*)a.vc + h * a.vhead);
-      // A row's place is worked out once, by one of 32 lanes a wave, and goes to the others through LDS; its table
-      // entry is loaded a tile before that, and looked at only then: nothing waits for it.
-      const int orow = wave * 16 + (lane & 15), okv = lane >> 4 & 1;
-      int entry = 0, slot = 0;
-      auto find = [&](int tile) { entry = page_entry(pages, min(tile * WIDE_TILE + orow, len - 1), slot); };
-      auto locate = [&](int tile) {
-        if (!good_page(pages, entry)) {  // reads page 0, and the sequence's rows become NaN
-          bad = true;
-          entry = 0;
-        }
-        const uint64_t at = okv ? cache_row(entry, slot, a.vpage, a.vslot) : cache_row(entry, slot, a.kpage, a.kslot);
-        if (lane < 32) offs[tile & 3][okv][orow] = at;
-      };
-      auto stage = [&](int tile, int kv) {
-        const uint32_t to = lds_at + kv * VBUF + (tile & 1) * TILE_BYTES + wave * 1024;  // the wave's 64 pieces in a row
-        for (int i = 0; i < PER; i++) {
-          const int row = prow + RPI * i, c = (pc ^ (kv ? vswz(row) : kswz(row))) * 8;
-          const char* p = (kv ? vc : kc) + offs[tile & 3][kv][row] + c * 2;
-          to_lds(c < a.D ? (const void*)p : &att_zero, to + i * ATT_BLOCK * 16);
-        }
-      };
-      if (tile < cached) {
-        find(tile);
-        locate(tile);
-        find(tile + 1);
-        locate(tile + 1);
-        find(tile + 2);
-        __syncthreads();
-        wait_loads();
-        stage(tile, 0);
-        stage(tile, 1);
-        if (tile + 1 < cached) stage(tile + 1, 0);
-        locate(tile + 2);
-        find(tile + 3);
-      }
+      const int parent = tree_parent(a.N, a.parents + b * a.parents_stride);  // (what does not hang on the length first)
       const T* q = (const T*)a.q + b * a.qs[0] + node * a.qs[1] + (h * G + m - node * G) * a.qs[2];
       for (int k = 0; k < KSTEPS; k++) {
         const int d = 16 * k + 8 * hh;
         qf[k] = m < M && d < a.D ? signed_by(*(const u32x4*)(q + d), a.scale) : att_zero;
       }
-      tree_paths(tr, a.N, a.parents + b * a.parents_stride);
+      const Pages pages = {a.table + b * a.table_stride, a.div, a.P, a.M};
+      const char* kc = (const char*)((const T*)a.kc + h * a.khead);
+      const char* vc = (const char*)((const T*)a.vc + h * a.vhead);
+      // A row's place is worked out once, by the lanes of one wave (the waves take turns), and goes to the others through
+      // LDS; its table entry is loaded four tiles before that, and looked at only then: nothing waits for it.
+      int entry = 0, slot = 0;
+      auto find = [&](int tile) { entry = page_entry(pages, min(tile * WIDE_TILE + lane, len - 1), slot); };
+      auto locate = [&](int tile) {
+        if (!good_page(pages, entry)) {  // reads page 0, and the sequence's rows become NaN
+          bad = true;
+          entry = 0;
+        }
+        offs[tile & 3][0][lane] = cache_row(entry, slot, a.kpage, a.kslot);
+        offs[tile & 3][1][lane] = cache_row(entry, slot, a.vpage, a.vslot);
+      };
+      // tiles t of the part are counted from its first: what is in LDS where goes by t & 1 and t & 3
+      auto stage = [&](int t, int kv, int buf) {
+        const uint32_t to = lds_at + kv * VBUF + buf * TILE_BYTES + wave * 1024;  // the wave's 64 pieces in a row
+        for (int i = 0; i < PER; i++) {
+          const int row = prow + RPI * i, c = (pc ^ (kv ? vswz(row) : kswz(row))) * 8;
+          const char* p = (kv ? vc : kc) + offs[t & 3][kv][row] + c * 2;
+          to_lds(FULL || c < a.D ? (const void*)p : &att_zero, to + i * ATT_BLOCK * 16);
+        }
+      };
+      const int n_cached = cached - tile;  // (of this part; at most 0 when it has the nodes alone)
+      if (n_cached > 0) {
+        find(first + wave);
+        if (wave < 3) {
+          locate(wave);
+          find(first + wave + 4);
+        }
+        __syncthreads();
+        wait_loads();
+        stage(0, 0, 0);
+        stage(0, 1, 0);
+        if (n_cached > 1) stage(1, 0, 1);
+      }
+      tree_paths(tr, a.N, parent);
 
       // The cache's tiles: a tile's scores are worked out while the weights of the one before it are, in the matrix
       // unit and beside it.  So K comes two tiles ahead and V one.
-      f32x16 s[2];
-      auto hide = [&](int tile) {  // key 32 c + 8 (i / 4) + 4 hh + i % 4 of the tile
-        if ((tile + 1) * WIDE_TILE <= len) return;
+      f32x16 s[2], n[2];
+      auto hide = [&](f32x16* s, int t) {  // key 32 c + 8 (i / 4) + 4 hh + i % 4 of the tile
+        const int base = (first + t) * WIDE_TILE;
+        if (base + WIDE_TILE <= len) return;
         for (int c = 0; c < 2; c++)
           for (int i = 0; i < 16; i++)
-            if (tile * WIDE_TILE + 32 * c + 8 * (i / 4) + 4 * hh + i % 4 >= len) s[c][i] = -INFINITY;
+            if (base + 32 * c + 8 * (i / 4) + 4 * hh + i % 4 >= len) s[c][i] = -INFINITY;
       };
-      if (tile < cached) {
-        wait_loads();
-        __syncthreads();
-        if (rows) {
-          scores(s, (tile & 1) * TILE_BYTES);
-          hide(tile);
-          follow(s);
-        }
-      }
-      for (; tile + 1 < cached; tile++) {
+      auto arrive = [&](int t, int buf) {
         wait_loads();     // this wave's pieces are in LDS
         __syncthreads();  // everyone's are; what the last tile was read from is free
-        locate(tile + 3);
-        find(tile + 4);
-        if (tile + 2 < cached) stage(tile + 2, 0);
-        stage(tile + 1, 1);
-        if (!rows) continue;
-        // In eight steps, each with products beside the exponentials of another step's weights.
-        const uint32_t vb = (tile & 1) * TILE_BYTES, kb = vb ^ TILE_BYTES;
+        if (wave == ((t + 3) & 3)) {
+          locate(t + 3);
+          find(first + t + 7);
+        }
+        if (t + 2 < n_cached) stage(t + 2, 0, buf);
+        if (t + 1 < n_cached) stage(t + 1, 1, buf ^ 1);
+      };
+      // tile t, whose scores are s, and the scores n of the next; in eight steps, each with products beside the
+      // exponentials of another step's weights
+      auto turn = [&](const f32x16* s, f32x16* n, int t, int buf) {
+        const uint32_t vb = buf * TILE_BYTES, kb = vb ^ TILE_BYTES;
         constexpr int KC = KSTEPS / 4;
         const float off = fmaf(-at_least(top), scale, Half<T>::bias);
         float part[2] = {0.f, 0.f};
-        f32x16 n[2];
         u32x4 p[4];
         auto keys = [&](int i) {
           for (int k = i * KC; k < (i + 1) * KC; k++)
             for (int c = 0; c < 2; c++) {
               const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-              n[c] = mfma32(lds_read<u32x4>(koff[k] + kb, c * 32 * CH * 16), qf[k], k ? n[c] : zero, T());
+              n[c] = mfma32(lds_read<u32x4>(koff[k], kb + c * 32 * CH * 16), qf[k], k ? n[c] : zero, T());
             }
         };
         auto values = [&](int st) {
           for (int d = 0; d < DB; d++) {
-            const u32x2 x = lds_read_tr(voff[d] + vb, 16 * st * CH * 16), y = lds_read_tr(voff[d] + vb, (16 * st + 8) * CH * 16);
+            const u32x2 x = lds_read_tr(voff[d], vb + 16 * st * CH * 16), y = lds_read_tr(voff[d], vb + (16 * st + 8) * CH * 16);
             o[d] = mfma32(u32x4{x[0], x[1], y[0], y[1]}, p[st], o[d], T());
           }
         };
@@ -689,20 +755,38 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
         then();
         values(3);
         sum += part[0] + part[1];
-        s[0] = n[0];
-        s[1] = n[1];
-        hide(tile + 1);
-        follow(s);
-      }
-      if (tile < cached) {
+        hide(n, t + 1);
+        follow(n);
+      };
+      if (n_cached > 0) {
         wait_loads();
         __syncthreads();
         if (rows) {
+          scores(s, 0);
+          hide(s, 0);
+          follow(s);
+        }
+        int t = 0;
+        for (; t + 2 < n_cached; t += 2) {
+          arrive(t, 0);
+          if (rows) turn(s, n, t, 0);
+          arrive(t + 1, 1);
+          if (rows) turn(n, s, t + 1, 1);
+        }
+        if (t + 1 < n_cached) {
+          arrive(t, 0);
+          if (rows) turn(s, n, t, 0);
+          t++;
+          s[0] = n[0];
+          s[1] = n[1];
+        }
+        arrive(t, t & 1);
+        if (rows) {
           u32x4 p[4];
           weigh(s, p);
-          product(p, (tile & 1) * TILE_BYTES);
+          product(p, (t & 1) * TILE_BYTES);
         }
-        tile++;
+        tile = cached;
       }
     }
 
@@ -818,9 +902,9 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend_join(AttendArgs a, int row
   const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + rows - 1) / rows, t = threadIdx.x;
   const int q = a.D / 4, each = ATT_BLOCK / (q * BY);  // rows a workgroup
   const int r = t / (q * BY), by = t / q % BY, d = t % q * 4;
-  const int64_t x = (int64_t)blockIdx.x * each + r;
-  const bool on = r < each && x < (int64_t)a.B * a.Hkv * M;
-  const int m = on ? (int)(x % M) : 0, bh = on ? (int)(x / M) : 0, h = bh % a.Hkv, b = bh / a.Hkv, n = m / G;
+  const uint32_t x = blockIdx.x * each + r;  // (the host keeps the rows below 2^31)
+  const bool on = r < each && x < (uint32_t)(a.B * a.Hkv * M);
+  const int bh = on ? (int)(x / (uint32_t)M) : 0, m = on ? (int)(x - bh * M) : 0, b = bh / a.Hkv, h = bh - b * a.Hkv, n = m / G;
   const int parts = on ? share_of(a, span_of(a, b, tile).tiles, 0).parts : 1;
   const float scale = score_scale(a.scale);
   const int64_t base = part_row(a, m / rows, bh, 0, rows, m % rows);

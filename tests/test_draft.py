@@ -394,7 +394,7 @@ extern "C" int split_ok(int d, int x) {
   page_split(page_div(d), x, k, s);
   return k == x / d && s == x % d;
 }
-extern "C" int depth(const int* par, int i) { return draft_depth(par, i); }
+extern "C" int path(const int* par, int i, uint32_t* w) { return draft_path(par, i, w); }
 """)
     so = d / "h.so"
     subprocess.run([shutil.which("g++"), "-O1", "-shared", "-fPIC", "-Wno-unknown-pragmas", "-fsanitize=undefined",
@@ -433,8 +433,11 @@ def test_tree_walk(host):
             par = np.array([-1] + [int(g.integers(0, i)) for i in range(1, N)], dtype=np.int32)
         if trial % 4 == 0:
             par[0] = -1
-        want = [-1 if x is None else len(x) - 1 for x in tree_paths(par.tolist())]
-        assert [host.depth(par.ctypes.data_as(ctypes.c_void_p), i) for i in range(N)] == want
+        w = (ctypes.c_uint32 * 4)()
+        for i, want in enumerate(tree_paths(par.tolist())):
+            here = host.path(par.ctypes.data_as(ctypes.c_void_p), i, w)
+            got = [j for j in range(128) if w[j // 32] >> j % 32 & 1]
+            assert bool(here) == (want is not None) and got == (want or [])
 
 
 # ---------------------------------------------------------------- GPU
@@ -453,6 +456,9 @@ ATTEND = [
     (4, 9, [5, 0, 77, 641], 14, 2, 120, 48, "chain"),
     (1, 2, [5000], 4, 1, 136, 16, "chain"),
     (70, 4, [i * 3 for i in range(70)], 4, 2, 64, 16, "random"),
+    (5, 3, [10, 900, 33, 0, 2000], 12, 1, 200, 16, "chain"),
+    (40, 5, [(i * 37) % 300 for i in range(40)], 16, 4, 64, 16, "chain"),
+    (30, 40, [(i * 97) % 2500 for i in range(30)], 16, 8, 64, 32, "random"),
 ]
 
 
