@@ -142,9 +142,11 @@ void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
     const int by = p.most > 16 && rows * (a.D / 4) < 512 * ATT_BLOCK && a.D <= 128 ? 8 : 1, each = ATT_BLOCK / (a.D / 4 * by);
     const dim3 joins((unsigned)((rows + each - 1) / each));
     if (by == 8)
-      hipLaunchKernelGGL((k_attend_join<T, 8>), joins, block, 0, s, a, p.rows, p.tile);
+      hipLaunchKernelGGL((k_attend_join<T, 8, 8>), joins, dim3(ATT_BLOCK), 0, s, a, p.rows, p.tile);
+    else if (p.most > 2)
+      hipLaunchKernelGGL((k_attend_join<T, 1, 8>), joins, dim3(ATT_BLOCK), 0, s, a, p.rows, p.tile);
     else
-      hipLaunchKernelGGL((k_attend_join<T, 1>), joins, block, 0, s, a, p.rows, p.tile);
+      hipLaunchKernelGGL((k_attend_join<T, 1, 2>), joins, dim3(ATT_BLOCK), 0, s, a, p.rows, p.tile);
   }
 }
 
@@ -252,7 +254,7 @@ int geobpe_commit_draft(int device, void* stream, const geobpe_commit_args* p) {
   if (x.layers < 1 || x.layers > 65535 || x.seqs < 0 || x.nodes < 1 || x.nodes > DRAFT_MAX_NODES || x.kv_heads < 1 ||
       x.kv_heads > 65535 || x.head_bytes < 16 || x.head_bytes > 65536 || x.head_bytes % 16 || x.page_size < 1 ||
       x.pages < 1 || x.max_pages < 0 || x.pages > INT32_MAX || x.page_size > DRAFT_MAX_POSITIONS ||
-      x.max_pages > DRAFT_MAX_POSITIONS / x.page_size || x.seqs > INT32_MAX / x.nodes)
+      x.max_pages > DRAFT_MAX_POSITIONS / x.page_size || x.seqs > INT32_MAX / 256 / x.nodes)
     return fail(GEOBPE_EARG, "commit: sizes out of range");
   if (x.seqs == 0) return GEOBPE_OK;
   if (!x.d_k || !x.d_v || !x.d_k_cache || !x.d_v_cache || !x.d_lens || !x.d_path || !x.d_n || !x.d_lens_out ||

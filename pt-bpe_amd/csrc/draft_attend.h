@@ -893,9 +893,9 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
   }
 }
 
-// Joins the parts: D / 4 threads a row, BY of them over its parts, eight parts in flight each.  Rows of sequences with
+// Joins the parts: D / 4 threads a row, BY of them over its parts, J parts in flight each.  Rows of sequences with
 // one part were written already.
-template <typename T, int BY>
+template <typename T, int BY, int J>
 __global__ __launch_bounds__(ATT_BLOCK) void k_attend_join(AttendArgs a, int rows, int tile) {
   __shared__ f32x4 acc_[BY > 1 ? ATT_BLOCK : 1];
   __shared__ float ml_[2][BY > 1 ? ATT_BLOCK : 1];
@@ -919,17 +919,18 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend_join(AttendArgs a, int row
     mx = up;
   };
   if (parts > 1)
-    for (int k = by; k < parts; k += 8 * BY) {
-      float m2[8], l2[8];
-      f32x4 v[8];
-      for (int j = 0; j < 8; j++) {
-        const int e = min(k + j * BY, parts - 1);
-        const int64_t at = base + (int64_t)e * rows;
+    for (int k = by; k < parts; k += J * BY) {
+      float m2[J], l2[J];
+      f32x4 v[J];
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        const int64_t at = base + (int64_t)min(k + j * BY, parts - 1) * rows;
         m2[j] = ml[2 * at];
         l2[j] = ml[2 * at + 1];
         v[j] = *(const f32x4*)(a.part + at * a.D + d);
       }
-      for (int j = 0; j < 8; j++)
+#pragma unroll
+      for (int j = 0; j < J; j++)
         if (k + j * BY < parts) add(m2[j], l2[j], v[j]);
     }
   if constexpr (BY > 1) {
