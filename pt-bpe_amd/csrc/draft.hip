@@ -50,11 +50,8 @@ bool aligned(const void* p, const int64_t* strides, int n, int64_t unit) {
 }
 
 // how a call is cut: rows a workgroup works on, tiles of keys a part has at most
-#ifndef WANT_S
-#define WANT_S 1024
-#endif
 struct AttendPlan {
-  bool wide, sorted;
+  bool wide;
   int rb, waves, rows, tile, per, most;
   int64_t row_tiles, blocks, bytes;
 };
@@ -63,19 +60,17 @@ AttendPlan attend_plan(const geobpe_attend_args& x) {
   const int64_t M = x.nodes * (x.heads / x.kv_heads);
   p.wide = M > (x.head_dim > 128 ? 16 : 32);
   p.rb = M <= 16 ? 1 : 2;
-  p.rows = p.wide ? WIDE_ROWS : 16 * p.rb;
+  p.rows = p.wide ? 32 * (M > 128 && x.head_dim > 64 && x.head_dim <= 128 ? 8 : 4) : 16 * p.rb;
   p.tile = p.wide ? WIDE_TILE : ATT_TILE;
   p.row_tiles = (M + p.rows - 1) / p.rows;
   const int64_t tiles = (x.max_pages * x.page_size + p.tile - 1) / p.tile + (x.nodes + p.tile - 1) / p.tile;
   const int64_t items = x.seqs * x.kv_heads;
   // eight waves where that fills the card without cutting the sequences (64 sequences x 4 heads: 26 us instead of 25 + 10
   // for the join); four where they are cut anyway, and more finely then (7 x 12 heads: 27 us instead of 40)
-  p.waves = !p.wide && x.head_dim <= 128 && items * p.row_tiles >= 128 && items * p.row_tiles <= 256 ? 8 : 4;
-  p.sorted = p.wide && x.seqs > 1 && x.seqs <= ATT_SORT;
-  const int64_t want = p.waves == 8 ? ATT_WANT / 2 : p.sorted ? WANT_S : ATT_WANT, even = (items * p.row_tiles * tiles + want - 1) / want;
+  p.waves = p.wide ? p.rows / 32 : x.head_dim <= 128 && items * p.row_tiles >= 128 && items * p.row_tiles <= 256 ? 8 : 4;
+  const int64_t want = ATT_WANT * 4 / p.waves, even = (items * p.row_tiles * tiles + want - 1) / want;
   p.per = (int)(even > tiles ? tiles : even > ATT_LEAST ? even : ATT_LEAST);
   p.most = (int)((tiles + p.per - 1) / p.per);
-  p.sorted = p.sorted && items * p.most * p.row_tiles > 512;
   p.blocks = (items * p.most + 7) / 8 * 8 * p.row_tiles;
   p.bytes = p.most > 1 ? items * p.row_tiles * p.most * p.rows * (x.head_dim + 2) * 4 : 0;
   return p;
@@ -113,18 +108,22 @@ void attend_narrow(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
 }
 template <typename T>
 void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.blocks), block(ATT_BLOCK);
+  const dim3 grid((unsigned)p.blocks), block(64 * p.waves);
   if (p.wide) {
     if (a.D == 64)
-      hipLaunchKernelGGL((k_attend_wide<T, 64, true>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((k_attend_wide<T, 64, true, 4>), grid, block, 0, s, a);
     else if (a.D < 64)
-      hipLaunchKernelGGL((k_attend_wide<T, 64, false>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((k_attend_wide<T, 64, false, 4>), grid, block, 0, s, a);
+    else if (a.D == 128 && p.waves == 8)
+      hipLaunchKernelGGL((k_attend_wide<T, 128, true, 8>), grid, block, 0, s, a);
     else if (a.D == 128)
-      hipLaunchKernelGGL((k_attend_wide<T, 128, true>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((k_attend_wide<T, 128, true, 4>), grid, block, 0, s, a);
+    else if (a.D < 128 && p.waves == 8)
+      hipLaunchKernelGGL((k_attend_wide<T, 128, false, 8>), grid, block, 0, s, a);
     else if (a.D < 128)
-      hipLaunchKernelGGL((k_attend_wide<T, 128, false>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((k_attend_wide<T, 128, false, 4>), grid, block, 0, s, a);
     else
-      hipLaunchKernelGGL((k_attend_wide<T, 256, false>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((k_attend_wide<T, 256, false, 4>), grid, block, 0, s, a);
   } else {
     switch ((a.D + 31) / 32) {
       case 1: attend_narrow<T, 1>(a, p, s); break;
@@ -208,7 +207,6 @@ int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p,
   a.scale = (float)x.scale;
   a.per = plan.per;
   a.most = plan.most;
-  a.sorted = plan.sorted;
   a.part = (float*)d_work;
   OnDevice on(device);
   if (!on.ok) return fail(GEOBPE_EHIP, "tree attention: device %d", device);

@@ -25,26 +25,18 @@ struct AttendArgs {
   PageDiv div;
   float scale;
   int32_t per, most;  // tiles a part of a sequence's keys has at most, parts there are room for
-  int32_t sorted;     // long parts first
   float* part;        // [row tile][item][part][row][D], then {max, sum} [row tile][item][part][row]
 };
 
 constexpr int ATT_BLOCK = 256;
 constexpr int ATT_WAVES = ATT_BLOCK / 64;
 constexpr int ATT_TILE = 32;  // keys a wave works on at a time
-// The keys are cut so that about two workgroups a CU have work (more parts cost their joining: at 512 / 1024 / 2048
-// workgroups 64 trees of 5 nodes over up to 2237 positions took 42 / 49 / 44 us, 32 of 64 nodes over up to 16 k 610 /
-// 631 / 656), but no part gets below 16 tiles (with 8 one token over 237 positions took 10.8 us instead of 8.2).
-#ifndef NSETS
-#define NSETS 1
-#endif
-#ifndef WANT
-#define WANT 512
-#define LEAST 16
-#endif
-constexpr int ATT_WANT = WANT, ATT_LEAST = LEAST;
-constexpr int ATT_SORT = ATT_BLOCK;  // sequences that are sorted at most
+// The keys are cut so that about two workgroups of four waves a CU have work (more parts cost their joining: at 512 / 1024
+// / 2048 workgroups 64 chains of 5 nodes over up to 2237 positions took 42 / 49 / 44 us when they were cut at all), but no
+// part gets below 16 tiles (with 8 one token over 237 positions took 10.8 us instead of 8.2).
+constexpr int ATT_WANT = 512, ATT_LEAST = 16;
 constexpr float LOG2E = 1.44269504088896340736f;
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -177,37 +169,6 @@ __device__ inline Share share_of(const AttendArgs& a, int tiles, int part) {
   s.last = min(s.first + size, tiles);
   return s;
 }
-// Which part of which item a workgroup has.  Sequences of different lengths are taken in the order of their parts'
-// sizes, the largest first, so that the last workgroups to start are short ones (32 x 64 nodes over 8 to 16 k
-// positions: see k_attend_wide).  Every workgroup works that out by itself, a thread a sequence.
-struct Work {
-  int b, h, part;
-};
-__device__ inline Work work_of(const AttendArgs& a, int work, int tile) {
-  if (!a.sorted) return {uni(work / a.most / a.Hkv), uni(work / a.most % a.Hkv), uni(work % a.most)};
-  __shared__ int size[ATT_SORT], count[ATT_SORT], found[2];
-  const int t = threadIdx.x;
-  int mine = 0;
-  if (t < a.B) {
-    const int tiles = span_of(a, t, tile).tiles;
-    const Share s = share_of(a, tiles, 0);
-    size[t] = mine = s.last;
-    count[t] = s.parts * a.Hkv;
-  }
-  if (t == 0) found[0] = -1;
-  __syncthreads();
-  if (t < a.B) {
-    int before = 0;
-    for (int b = 0; b < a.B; b++)
-      if (size[b] > mine || (size[b] == mine && b < t)) before += count[b];
-    if (work >= before && work < before + count[t]) {
-      found[0] = t;
-      found[1] = work - before;
-    }
-  }
-  __syncthreads();
-  return {uni(found[0]), uni(found[1] % a.Hkv), uni(found[1] / a.Hkv)};
-}
 // a row's place among the parts
 __device__ inline int64_t part_row(const AttendArgs& a, int rt, int item, int part, int rows, int row) {
   return (((int64_t)rt * a.B * a.Hkv + item) * a.most + part) * rows + row;
@@ -227,7 +188,7 @@ __device__ inline float* part_sums(const AttendArgs& a, int RT, int rows) {
 template <typename T, int KS, int RB, int W>
 __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 : 1) void k_attend(AttendArgs a) {
   constexpr int DP = 32 * KS, DB = 2 * KS, LROW = DP * 2 + 32;
-  constexpr int DMIN = KS <= 4 ? DP - 24 : DP - 56, SETS = KS <= 4 ? NSETS : 1;  // the heads this is for: DMIN .. DP
+  constexpr int DMIN = KS <= 4 ? DP - 24 : DP - 56;  // the heads this is for: DMIN .. DP
   constexpr int AREA = ATT_TILE * LROW;  // >= 16 rows of DP + 4 floats
   __shared__ __attribute__((aligned(16))) char lds[W * AREA];
   __shared__ Tree tr;
@@ -272,12 +233,12 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
   struct Tile {
     u32x4 k[2][KS], v[2][KS];
     int id[2], slot[2];
-  };
-  auto find = [&](Tile& x, int tile) {
+  } x;
+  auto find = [&](int tile) {
     for (int c = 0; c < 2; c++)
       x.id[c] = page_entry(pages, min(tile * ATT_TILE + 16 * c + l4, sp.len - 1), x.slot[c]);
   };
-  auto load = [&](Tile& x, int c, const T* kp, const T* vp) {
+  auto load = [&](int c, const T* kp, const T* vp) {
     for (int k = 0; k < KS; k++) {
       const int d = 32 * k + 8 * p4;
       if (32 * k + 32 <= DMIN) {
@@ -291,24 +252,24 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
       }
     }
   };
-  auto fetch = [&](Tile& x) {
+  auto fetch = [&]() {
     for (int c = 0; c < 2; c++) {
       if (!good_page(pages, x.id[c])) {  // reads page 0, and the sequence's rows become NaN
         bad = true;
         x.id[c] = 0;
       }
-      load(x, c, (const T*)(kc + cache_row(x.id[c], x.slot[c], a.kpage, a.kslot)),
+      load(c, (const T*)(kc + cache_row(x.id[c], x.slot[c], a.kpage, a.kslot)),
            (const T*)(vc + cache_row(x.id[c], x.slot[c], a.vpage, a.vslot)));
     }
   };
-  // SETS tiles of a wave are on their way at a time
+  // one tile of a wave is on its way while another is worked on (with two on their way nothing got faster: 25.5 us
+  // against 24.7, and 40 against 27 where the registers then hold one workgroup a CU)
   const int cached = min(last, sp.cache_tiles);
   int tile = first + wave;
-  Tile x[SETS];
   if (tile < cached) {
-    for (int i = 0; i < SETS; i++) find(x[i], tile + i * W);
-    for (int i = 0; i < SETS; i++) fetch(x[i]);
-    for (int i = 0; i < SETS; i++) find(x[i], tile + (SETS + i) * W);
+    find(tile);
+    fetch();
+    find(tile + W);
   }
   tree_paths(tr, a.N, parent);
 
@@ -319,7 +280,7 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
     sum[r] = 0.f;
     for (int d = 0; d < DB; d++) o[d][r] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  auto step = [&](auto is_nodes, int base, Tile& x, int tile) {
+  auto step = [&](auto is_nodes, int base) {
     constexpr bool nodes = decltype(is_nodes)::value;
     // K into the operands' order through the wave's LDS, then V there for the transposing read
     char* mine = area + l4 * LROW + p4 * 16;
@@ -349,9 +310,9 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
         s[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < KS; k++) s[c][r] = Half<T>::mfma(kf[c][k], qf[r][k], s[c][r]);
       }
-    if (!nodes && tile + SETS * W < cached) {
-      fetch(x);
-      find(x, tile + 2 * SETS * W);
+    if (!nodes && tile + W < cached) {
+      fetch();
+      find(tile + 2 * W);
     }
     u32x4 p[RB];
     for (int r = 0; r < RB; r++) {
@@ -431,22 +392,14 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
       wave_order();
     }
   };
-  while (tile < cached) {
-#pragma unroll
-    for (int i = 0; i < SETS; i++) {
-      if (tile < cached) {
-        step(std::false_type(), tile * ATT_TILE, x[i], tile);
-        tile += W;
-      }
-    }
-  }
+  for (; tile < cached; tile += W) step(std::false_type(), tile * ATT_TILE);
   for (; tile < last; tile += W) {
     const int base = (tile - sp.cache_tiles) * ATT_TILE;
     for (int c = 0; c < 2; c++) {
       const int n = min(base + 16 * c + l4, a.N - 1);
-      load(x[0], c, kd + n * a.kds[1], vd + n * a.vds[1]);
+      load(c, kd + n * a.kds[1], vd + n * a.vds[1]);
     }
-    step(std::true_type(), base, x[0], tile);
+    step(std::true_type(), base);
   }
 
   // the waves' sums joined: maxima first, then 16 rows at a time through LDS
@@ -496,7 +449,7 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
 }
 
 // ---- many rows -------------------------------------------------------------------------------
-// Above 32 rows a kv head the keys are shared: a workgroup has 128 rows, 32 a wave, and its waves read the same
+// Above 32 rows a kv head the keys are shared: a workgroup has 128 or 256 rows, 32 a wave, and its waves read the same
 // tiles of 64 keys from LDS.  The cache's rows go there directly, the next tile's while this one's products run.
 // S^T = K Q^T and O^T = V^T P^T in the 32x32x16 instruction, in the same way as above: row = lane % 32, and a
 // lane's weights of four keys in a row are the second product's operand.
@@ -505,7 +458,6 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
 // row r lies at c ^ (r & 7) (eight rows, one piece each), V's at c ^ 4 (r & 3) (four rows, 64 bytes each; rows of
 // 128 bytes: c ^ 4 (r / 2 & 1)).
 constexpr int WIDE_TILE = 64;
-constexpr int WIDE_ROWS = 128;
 constexpr float SLACK = 8.f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -551,11 +503,12 @@ __device__ inline void wait_loads() {
 
 __device__ const u32x4 att_zero = {0, 0, 0, 0};  // what a head's pieces past its end are read from
 
-template <typename T, int DP, bool FULL>
-__global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(AttendArgs a) {
+template <typename T, int DP, bool FULL, int W>
+__global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(AttendArgs a) {
+  constexpr int BLOCK = 64 * W, ROWS = 32 * W;
   constexpr int CH = DP / 8, KSTEPS = DP / 16, DB = DP / 32;
-  constexpr int TILE_BYTES = WIDE_TILE * DP * 2, PER = WIDE_TILE * CH / ATT_BLOCK;  // pieces a thread moves
-  constexpr int RPI = ATT_BLOCK / CH;                                               // rows between them
+  constexpr int TILE_BYTES = WIDE_TILE * DP * 2, PER = WIDE_TILE * CH / BLOCK;  // pieces a thread moves
+  constexpr int RPI = BLOCK / CH;                                               // rows between them
   constexpr uint32_t VBUF = 2 * TILE_BYTES;
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];  // K of two tiles, V of two
   __shared__ uint64_t offs[4][2][WIDE_TILE];                         // the rows' places in the cache: tile % 4, K or V
@@ -564,18 +517,16 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, hh = lane >> 5;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   const float scale = score_scale(a.scale);
-  const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + WIDE_ROWS - 1) / WIDE_ROWS;
+  const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + ROWS - 1) / ROWS;
   const int die = blockIdx.x & 7, j8 = blockIdx.x >> 3;
   const int rt = uni(j8 % RT), work = uni((j8 / RT) * 8 + die);
   if (work >= a.B * a.Hkv * a.most) return;
-  const Work wk = work_of(a, work, WIDE_TILE);
-  if (wk.b < 0) return;
-  const int b = wk.b, h = wk.h, part = wk.part, item = b * a.Hkv + h;
+  const int part = uni(work % a.most), item = uni(work / a.most), h = uni(item % a.Hkv), b = uni(item / a.Hkv);
   const Span sp = span_of(a, b, WIDE_TILE);
   const Share sh = share_of(a, sp.tiles, part);
   if (part >= sh.parts) return;
-  const int m = rt * WIDE_ROWS + wave * 32 + l32, node = m / G;
-  const bool rows = rt * WIDE_ROWS + uni(wave) * 32 < M;  // (the wave has any)
+  const int m = rt * ROWS + wave * 32 + l32, node = m / G;
+  const bool rows = rt * ROWS + uni(wave) * 32 < M;  // (the wave has any)
 
   // where this lane's operands lie in a tile: K's piece 2 k + hh of row l32, V's four keys of 16 channels
   auto kswz = [](int row) { return row & 7 & (CH - 1); };
@@ -670,7 +621,7 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
         for (int i = 0; i < PER; i++) {
           const int row = prow + RPI * i, c = (pc ^ (kv ? vswz(row) : kswz(row))) * 8;
           const char* p = (kv ? vc : kc) + offs[t & 3][kv][row] + c * 2;
-          to_lds(FULL || c < a.D ? (const void*)p : &att_zero, to + i * ATT_BLOCK * 16);
+          to_lds(FULL || c < a.D ? (const void*)p : &att_zero, to + i * BLOCK * 16);
         }
       };
       const int n_cached = cached - tile;  // (of this part; at most 0 when it has the nodes alone)
@@ -807,8 +758,8 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
           v = att_zero;
           odd_ = 1;
         }
-        *(u32x4*)(lds + (t + ATT_BLOCK * i) * 16) = k;
-        *(u32x4*)(lds + VBUF + (t + ATT_BLOCK * i) * 16) = v;
+        *(u32x4*)(lds + (t + BLOCK * i) * 16) = k;
+        *(u32x4*)(lds + VBUF + (t + BLOCK * i) * 16) = v;
       }
       __syncthreads();
       if (!rows) continue;
@@ -824,14 +775,15 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
       weigh(s, p);
       product(p, 0);
       if (!odd_) continue;
-      // the sums of what went in as 0 (the finite values of its pieces with their weights), half the channels at a time,
+      // the sums of what went in as 0 (the finite values of its pieces with their weights), some of the channels at a time,
       // in the LDS that the tile does not use
+      constexpr int TURNS = W / 2, DT = DP / TURNS;
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int slice = wave * 32 + l32, d0 = half * (DP / 2);
-        float* mine = (float*)(lds + (slice < WIDE_ROWS / 2 ? TILE_BYTES : VBUF + TILE_BYTES)) + slice % (WIDE_ROWS / 2) * (DP / 2);
+      for (int turn = 0; turn < TURNS; turn++) {
+        const int slice = wave * 32 + l32, d0 = turn * DT;
+        float* mine = (float*)(lds + (slice < ROWS / 2 ? TILE_BYTES : VBUF + TILE_BYTES)) + slice % (ROWS / 2) * DT;
 #pragma unroll 1
-        for (int d = 4 * hh; d < DP / 2; d += 8) *(f32x4*)(mine + d) = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int d = 4 * hh; d < DT; d += 8) *(f32x4*)(mine + d) = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int j = 0; j < WIDE_TILE && base + j < a.N; j++) {
           if (m >= M || !(tr.anc[node][(base + j) / 32] >> (j % 32) & 1)) continue;
@@ -843,7 +795,7 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
           for (int e = 0; e < a.D; e++) dot = fmaf((float)q[e], (float)k[e], dot);
           const float w = __builtin_amdgcn_exp2f(fmaf((a.scale < 0.f ? -dot : dot) - at_least(top), scale, Half<T>::bias));
 #pragma unroll 1
-          for (int d = 4 * hh; d < DP / 2 && d0 + d < a.D; d += 8) {
+          for (int d = 4 * hh; d < DT && d0 + d < a.D; d += 8) {
             if (!not_finite<T>(*(const u32x4*)(v + (d0 + d) / 8 * 8))) continue;
             for (int i = 0; i < 4; i++) {
               const float y = (float)v[d0 + d + i];
@@ -853,15 +805,12 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
         }
         wave_order();
 #pragma unroll
-        for (int d = 0; d < DB / 2; d++)
+        for (int d = 0; d < DT / 32; d++)
+#pragma unroll
           for (int i = 0; i < 4; i++) {
             const f32x4 x = *(const f32x4*)(mine + 32 * d + 8 * i + 4 * hh);
-            for (int e = 0; e < 4; e++) {
-              if (half == 0)
-                o[d][4 * i + e] += x[e];
-              else
-                o[DB / 2 + d][4 * i + e] += x[e];
-            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[turn * (DT / 32) + d][4 * i + e] += x[e];
           }
         wave_order();
       }
@@ -870,12 +819,12 @@ __global__ __launch_bounds__(ATT_BLOCK, DP > 128 ? 1 : 2) void k_attend_wide(Att
     sum += __shfl_xor(sum, 32);
     if (__syncthreads_or(bad)) sum = NAN;
     if (m < M) {
-      const int64_t at = part_row(a, rt, item, part, WIDE_ROWS, wave * 32 + l32);
+      const int64_t at = part_row(a, rt, item, part, ROWS, wave * 32 + l32);
       const bool here = tr.anc[node][node / 32] >> (node % 32) & 1;
       const float f = 1.f / sum;
       T* out = (T*)a.out + (((int64_t)b * a.N + node) * a.Hq + h * G + m - node * G) * a.D;
       if (sh.parts > 1 && hh == 0) {
-        float* ml = part_sums(a, RT, WIDE_ROWS) + 2 * at;
+        float* ml = part_sums(a, RT, ROWS) + 2 * at;
         ml[0] = here ? top : -INFINITY;
         ml[1] = here ? sum : 0.f;
       }

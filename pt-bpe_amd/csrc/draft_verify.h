@@ -35,9 +35,9 @@ struct VerifyArgs {
 };
 
 constexpr int VER_MAX_VOCAB = 1 << 22;
-#ifndef VER_SMALL
-#define VER_SMALL 8192
-#endif
+// up to here four waves do a sequence, above 16 (48 trees of 40 nodes over 5123 ids: 14.0 us with four, 16.7 with 16)
+constexpr int VER_SMALL = 8192;
+// a sum that falls below this part of itself by subtraction is taken anew: the rest keeps 33 bits and more
 constexpr double VER_KEEP = 1.0 / (1 << 20);
 
 // 16 bytes of a row that is aligned to its elements only
