@@ -273,7 +273,8 @@ int geobpe_commit_draft(int device, void* stream, const geobpe_commit_args* p) {
   a.div = page_div(a.S);
   OnDevice on(device);
   if (!on.ok) return fail(GEOBPE_EHIP, "commit: device %d", device);
-  hipLaunchKernelGGL(k_commit_nodes, dim3((unsigned)(a.B * a.N), (unsigned)a.L), dim3(256), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(k_commit_nodes, dim3((unsigned)(a.B * a.N), (unsigned)((a.L + COMMIT_LAYERS - 1) / COMMIT_LAYERS)),
+                     dim3(256), 0, (hipStream_t)stream, a);
   return launched("commit");
 }
 

@@ -20,15 +20,16 @@ struct CommitArgs {
   PageDiv div;
 };
 
-struct alignas(16) Piece {
-  uint32_t v[4];
-};
+typedef uint32_t Piece __attribute__((ext_vector_type(4)));  // 16 bytes
 
-// One workgroup per kept node and layer.  Measured against it: four layers a workgroup (3.1 us became 4.3 for one sequence,
-// 64 sequences x 16 layers stayed at 27), four nodes a workgroup with one die for all of a sequence's layer (4.8, 28).
-// What bounds the large case is not in here: 17 k rows of 2 KiB go to 4 k different places of 2 MiB each.
+// One workgroup per kept node and COMMIT_LAYERS layers, half of it for the keys and half for the values; a thread has
+// one piece of every one of its layers on its way at a time.  Stores past the caches, for what is written is not read
+// before the whole cache is.  64 sequences x 16 layers of 2 KiB rows, 71 MB read and written: with 1 / 2 / 4 / 8 / 16
+// layers a workgroup 23 / 16 / 15.5 / 17 / 22 us, a copy's rate would be 14; with stores through the caches 27 at 1
+// layer.  One sequence x 6 layers: 6.9 us with any, the call itself.
+constexpr int COMMIT_LAYERS = 4;
 __global__ __launch_bounds__(256) void k_commit_nodes(CommitArgs a) {
-  const int b = blockIdx.x / a.N, t = blockIdx.x - b * a.N, layer = blockIdx.y;
+  const int b = blockIdx.x / a.N, t = blockIdx.x - b * a.N, layer = blockIdx.y * COMMIT_LAYERS;
   const int len = a.lens[b], n = min(a.n[b], a.N);
   // a kept node outside the tree or the cache is not written, and the sequence's length becomes -1
   const Pages pages = {a.table + b * a.table_stride, a.div, a.P, a.M};
@@ -46,12 +47,22 @@ __global__ __launch_bounds__(256) void k_commit_nodes(CommitArgs a) {
     if (threadIdx.x == 0) a.lens_out[b] = ok ? len + max(n, 0) : -1;
   }
   if (t >= n || !place(t, node, id, slot)) return;
-  for (int k = threadIdx.x; k < a.Hkv * a.vecs; k += 256) {
+  const bool values = threadIdx.x >= 128;
+  const int64_t* ds = values ? a.vds : a.kds;
+  const int64_t* cs = values ? a.vcs : a.kcs;
+  const char* from = (values ? a.vd : a.kd) + layer * ds[0] + b * ds[1] + node * ds[2];
+  char* to = (values ? a.vc : a.kc) + layer * cs[0] + id * cs[1] + slot * cs[2];
+  const int64_t dl = ds[0], cl = cs[0], dh = ds[3], ch = cs[3];
+  const int layers = min(COMMIT_LAYERS, a.L - layer);
+  for (int k = threadIdx.x & 127; k < a.Hkv * a.vecs; k += 128) {
     const int h = k / a.vecs, c = (k - h * a.vecs) * 16;
-    const Piece x = *(const Piece*)(a.kd + layer * a.kds[0] + b * a.kds[1] + node * a.kds[2] + h * a.kds[3] + c);
-    const Piece y = *(const Piece*)(a.vd + layer * a.vds[0] + b * a.vds[1] + node * a.vds[2] + h * a.vds[3] + c);
-    *(Piece*)(a.kc + layer * a.kcs[0] + id * a.kcs[1] + slot * a.kcs[2] + h * a.kcs[3] + c) = x;
-    *(Piece*)(a.vc + layer * a.vcs[0] + id * a.vcs[1] + slot * a.vcs[2] + h * a.vcs[3] + c) = y;
+    Piece x[COMMIT_LAYERS];
+#pragma unroll
+    for (int l = 0; l < COMMIT_LAYERS; l++)
+      if (l < layers) x[l] = *(const Piece*)(from + l * dl + h * dh + c);
+#pragma unroll
+    for (int l = 0; l < COMMIT_LAYERS; l++)
+      if (l < layers) __builtin_nontemporal_store(x[l], (Piece*)(to + l * cl + h * ch + c));
   }
 }
 
