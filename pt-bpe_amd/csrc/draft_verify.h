@@ -80,13 +80,30 @@ struct VerRow {
     }
   }
   __device__ void values(const Raw& w, int i, double* r) const {
+    // entries that are no probabilities are rare: looked for all at once, as the bits above the largest finite value's
+    float pv[VEC], qv[VEC];
+    uint32_t top = 0;
 #pragma unroll
-    for (int k = 0; k < VEC; k++) r[k] = prob(w.p.v[k]);
+    for (int k = 0; k < VEC; k++) {
+      pv[k] = (float)w.p.v[k];
+      qv[k] = two() ? (float)w.q.v[k] : 0.f;
+      top = max(max(top, __float_as_uint(pv[k])), __float_as_uint(qv[k]));
+    }
+    if (__any(top > 0x7f7fffffu)) {
+#pragma unroll
+      for (int k = 0; k < VEC; k++) pv[k] = prob(pv[k]), qv[k] = prob(qv[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; k++) r[k] = pv[k];
     if (Q) {
-      for (int j = 0; j < rejected; j++) {
+      if (rejected) {  // (Z of the first is 1)
+#pragma unroll
+        for (int k = 0; k < VEC; k++) r[k] = fmax(r[k] - (double)qv[k], 0.0);
+      }
+      for (int j = 1; j < rejected; j++) {
         const double z = Z[j];
 #pragma unroll
-        for (int k = 0; k < VEC; k++) r[k] = fmax(r[k] - z * (double)prob(w.q.v[k]), 0.0);
+        for (int k = 0; k < VEC; k++) r[k] = fmax(fma(-z, (double)qv[k], r[k]), 0.0);
       }
     } else {
       for (int j = 0; j < rejected; j++)
@@ -257,7 +274,7 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
           seen = row.rejected;
         }
         if (Q) {
-          for (int j = 0; j < row.rejected; j++) r = fmax(r - Z[j] * qx, 0.0);
+          for (int j = 0; j < row.rejected; j++) r = fmax(fma(-Z[j], qx, r), 0.0);
         } else {
           if (__ballot((gone[0] >> lane & 1) && id[0] == x) | __ballot((gone[1] >> lane & 1) && id[1] == x)) r = 0;
         }
