@@ -220,7 +220,7 @@ int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p,
 int geobpe_verify_draft(int device, void* stream, const geobpe_verify_args* p) {
   if (!p) return fail(GEOBPE_EARG, "no arguments");
   const geobpe_verify_args& x = *p;
-  if (x.seqs < 0 || x.seqs > INT32_MAX || x.nodes < 1 || x.nodes > DRAFT_MAX_NODES || x.vocab < 1 ||
+  if (x.seqs < 0 || x.seqs > INT32_MAX / 1024 || x.nodes < 1 || x.nodes > DRAFT_MAX_NODES || x.vocab < 1 ||
       x.vocab > VER_MAX_VOCAB || x.classes < 0 || x.classes > INT32_MAX || x.dtype < 0 || x.dtype > 2)
     return fail(GEOBPE_EARG, "verify: sizes out of range");
   if (x.seqs == 0) return GEOBPE_OK;

@@ -29,7 +29,6 @@ struct AttendArgs {
 };
 
 constexpr int ATT_BLOCK = 256;
-constexpr int ATT_WAVES = ATT_BLOCK / 64;
 constexpr int ATT_TILE = 32;  // keys a wave works on at a time
 // The keys are cut so that about two workgroups of four waves a CU have work (more parts cost their joining: at 512 / 1024
 // / 2048 workgroups 64 chains of 5 nodes over up to 2237 positions took 42 / 49 / 44 us when they were cut at all), but no
@@ -109,6 +108,11 @@ __device__ inline void wave_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
+__device__ inline u32x4 keep_if(bool in, u32x4 y) {
+  for (int i = 0; i < 4; i++) y[i] = in ? y[i] : 0u;
+  return y;
+}
+
 // exponent all ones in any of the eight halves
 template <typename T>
 __device__ inline bool not_finite(u32x4 v) {
@@ -182,9 +186,9 @@ __device__ inline float* part_sums(const AttendArgs& a, int RT, int rows) {
 //
 // S^T = K Q^T and O^T = V^T P^T in the 16x16x32 matrix instruction: a lane then holds its own row's
 // weights (row = lane % 16), running maximum and sums, and the weights of four keys in a row are what the second
-// product's operand wants, so nothing is moved between lanes but the maximum.  K goes from memory into the operand
-// registers, V through the wave's own LDS, where the transposing read turns it; the rows there are 32 bytes longer
-// than the head so that eight of them start in different banks.
+// product's operand wants, so nothing is moved between lanes but the maximum.  K and then V go through the wave's own
+// LDS: K to be read in the operand's order, V for the transposing read; the rows there are 32 bytes longer than the head
+// so that eight of them start in different banks.
 template <typename T, int KS, int RB, int W>
 __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 : 1) void k_attend(AttendArgs a) {
   constexpr int DP = 32 * KS, DB = 2 * KS, LROW = DP * 2 + 32;
@@ -246,8 +250,7 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
         x.v[c][k] = *(const u32x4*)(vp + d);
       } else {  // (past the head: K is 0 there, as the query is; V's channels there go nowhere)
         const bool in = d < a.D;
-        const u32x4 y = *(const u32x4*)(kp + (in ? d : 0));
-        for (int i = 0; i < 4; i++) x.k[c][k][i] = in ? y[i] : 0u;
+        x.k[c][k] = keep_if(in, *(const u32x4*)(kp + (in ? d : 0)));
         x.v[c][k] = *(const u32x4*)(vp + (in ? d : 0));
       }
     }
@@ -291,6 +294,11 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
     for (int c = 0; c < 2; c++)
       for (int k = 0; k < KS; k++) kf[c][k] = *(const u32x4*)(area + (16 * c + l16) * LROW + k * 64 + lq * 16);
     wave_order();
+    if constexpr (!nodes) {
+      if (base + ATT_TILE > sp.len)  // (behind the last position it is loaded again: its value there has to be 0)
+        for (int c = 0; c < 2; c++)
+          for (int k = 0; k < KS; k++) x.v[c][k] = keep_if(base + 16 * c + l4 < sp.len, x.v[c][k]);
+    }
     bool odd = false;  // a node's value that is not finite
     for (int c = 0; c < 2; c++)
       for (int k = 0; k < KS; k++) {
@@ -299,7 +307,7 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
           // such values go in as 0 and are added below where they belong
           const bool bad_v = not_finite<T>(x.v[c][k]);
           odd |= bad_v;
-          for (int i = 0; i < 4; i++) x.v[c][k][i] = bad_v ? 0u : x.v[c][k][i];
+          x.v[c][k] = keep_if(!bad_v, x.v[c][k]);
         }
         *(u32x4*)(mine + c * 16 * LROW + k * 64) = x.v[c][k];
       }
@@ -501,7 +509,8 @@ __device__ inline void wait_loads() {
   asm volatile("" ::: "memory");
 }
 
-__device__ const u32x4 att_zero = {0, 0, 0, 0};  // what a head's pieces past its end are read from
+// what a head's pieces past its end and the values behind the last position are read from
+__device__ const u32x4 att_zero[32] = {};
 
 template <typename T, int DP, bool FULL, int W>
 __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(AttendArgs a) {
@@ -598,7 +607,10 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
       const T* q = (const T*)a.q + b * a.qs[0] + node * a.qs[1] + (h * G + m - node * G) * a.qs[2];
       for (int k = 0; k < KSTEPS; k++) {
         const int d = 16 * k + 8 * hh;
-        qf[k] = m < M && d < a.D ? signed_by(*(const u32x4*)(q + d), a.scale) : att_zero;
+        if (m < M && d < a.D)
+          qf[k] = signed_by(*(const u32x4*)(q + d), a.scale);
+        else
+          qf[k] = u32x4{0, 0, 0, 0};
       }
       const Pages pages = {a.table + b * a.table_stride, a.div, a.P, a.M};
       const char* kc = (const char*)((const T*)a.kc + h * a.khead);
@@ -613,7 +625,8 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
           entry = 0;
         }
         offs[tile & 3][0][lane] = cache_row(entry, slot, a.kpage, a.kslot);
-        offs[tile & 3][1][lane] = cache_row(entry, slot, a.vpage, a.vslot);
+        offs[tile & 3][1][lane] = (first + tile) * WIDE_TILE + lane < len ? cache_row(entry, slot, a.vpage, a.vslot)
+                                                                          : (uint64_t)((const char*)att_zero - vc);
       };
       // tiles t of the part are counted from its first: what is in LDS where goes by t & 1 and t & 3
       auto stage = [&](int t, int kv, int buf) {
@@ -621,7 +634,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
         for (int i = 0; i < PER; i++) {
           const int row = prow + RPI * i, c = (pc ^ (kv ? vswz(row) : kswz(row))) * 8;
           const char* p = (kv ? vc : kc) + offs[t & 3][kv][row] + c * 2;
-          to_lds(FULL || c < a.D ? (const void*)p : &att_zero, to + i * BLOCK * 16);
+          to_lds(FULL || c < a.D ? (const void*)p : att_zero, to + i * BLOCK * 16);
         }
       };
       const int n_cached = cached - tile;  // (of this part; at most 0 when it has the nodes alone)
@@ -752,12 +765,10 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
       for (int i = 0; i < PER; i++) {
         const int row = prow + RPI * i, n = min(base + row, a.N - 1);
         const int ck = (pc ^ kswz(row)) * 8, cv = (pc ^ vswz(row)) * 8;
-        const u32x4 k = ck < a.D ? *(const u32x4*)(kd + n * a.kds[1] + ck) : att_zero;
-        u32x4 v = cv < a.D ? *(const u32x4*)(vd + n * a.vds[1] + cv) : att_zero;
-        if (not_finite<T>(v)) {
-          v = att_zero;
-          odd_ = 1;
-        }
+        const u32x4 k = keep_if(ck < a.D, *(const u32x4*)(kd + n * a.kds[1] + (ck < a.D ? ck : 0)));
+        u32x4 v = keep_if(cv < a.D, *(const u32x4*)(vd + n * a.vds[1] + (cv < a.D ? cv : 0)));
+        if (not_finite<T>(v)) odd_ = 1;
+        v = keep_if(!not_finite<T>(v), v);
         *(u32x4*)(lds + (t + BLOCK * i) * 16) = k;
         *(u32x4*)(lds + VBUF + (t + BLOCK * i) * 16) = v;
       }

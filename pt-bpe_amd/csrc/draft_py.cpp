@@ -45,7 +45,10 @@ std::string shape_of(const at::Tensor& x) {
 const at::Tensor& tensor(const char* name, PyObject* o) {
   if (!THPVariable_Check(o))
     refuse(PyExc_TypeError, "%s: a torch tensor is expected, not %s", name, Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
+  const at::Tensor& x = THPVariable_Unpack(o);
+  if (x.is_conj() || x.is_neg())
+    VALUE("%s is a view that negates or conjugates: pass %s.resolve_conj().resolve_neg()", name, name);
+  return x;
 }
 
 // x as an operand: its type, its device, its shape (-1: any size)
@@ -84,6 +87,19 @@ void rows(const char* name, const at::Tensor& x, int64_t* out, int64_t scale) {
     out[i] = s * e / scale;
   }
   if (!ok) VALUE("%s: rows must be contiguous and 16-byte aligned: pass %s.contiguous()", name, name);
+}
+
+// whether two tensors' spans of memory meet
+bool meet(const at::Tensor& x, const at::Tensor& y) {
+  const at::Tensor* t[2] = {&x, &y};
+  uintptr_t from[2], to[2];
+  for (int i = 0; i < 2; i++) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t[i]->dim(); d++) last += (t[i]->size(d) - 1) * t[i]->stride(d);
+    from[i] = (uintptr_t)t[i]->data_ptr();
+    to[i] = t[i]->numel() ? from[i] + (last + 1) * t[i]->element_size() : from[i];
+  }
+  return from[0] < to[1] && from[1] < to[0];
 }
 
 bool unit(const at::Tensor& x) { return x.size(-1) <= 1 || x.stride(-1) == 1; }
@@ -296,6 +312,10 @@ PyObject* commit(PyObject*, PyObject* const* o, Py_ssize_t nargs) {
     for (int64_t d = 0; i > 1 && d < all[i]->dim(); d++)
       if (all[i]->stride(d) == 0 && all[i]->size(d) > 1) VALUE("%s is expanded: its rows share memory", names[i]);
   }
+  for (int i = 0; i < 2; i++)
+    if (meet(*x[i], *c.k) || meet(*x[i], *c.v))
+      VALUE("%s lies in the cache's own memory, which the call writes: pass %s.clone()", names[i], names[i]);
+  if (c.k->data_ptr() == c.v->data_ptr()) VALUE("v_cache is k_cache: each needs memory of its own");
   const hipStream_t stream = stream_of(dev);
   at::Tensor out = at::empty({c.B}, c.lens->options());
   a.d_k = x[0]->data_ptr(), a.d_v = x[1]->data_ptr(), a.d_k_cache = c.k->data_ptr(), a.d_v_cache = c.v->data_ptr();

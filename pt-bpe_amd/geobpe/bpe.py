@@ -509,10 +509,10 @@ class BPE:
         device = torch.device(device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        kept = getattr(self, "_id_ranges", None)
-        if kept is None or kept[0] != (K, device):
-            kept = self._id_ranges = ((K, device), torch.tensor(r, device=device))
-        return kept[1]
+        kept = self.__dict__.setdefault("_id_ranges", {})
+        if (K, device) not in kept:
+            kept[K, device] = torch.tensor(r, device=device)
+        return kept[K, device]
 
     def verify_draft(self, parents, ids, target, draft, u, start):
         """Drafted ids against a model's probabilities over this vocabulary (geobpe.draft.verify), each place

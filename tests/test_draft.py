@@ -324,6 +324,13 @@ def test_commit_refusals():
     refuse(commit, c, TypeError, "path", path=c["path"].long())
     refuse(commit, c, ValueError, "n:", n=c["n"][:2])
     refuse(commit, c, ValueError, "expanded", k_cache=c["k_cache"][:1].expand(2, -1, -1, -1, -1))
+    both = torch.zeros(2, 20, 4, 2, 16, dtype=BF)
+    P = c["k_cache"].shape[1]
+    refuse(commit, c, ValueError, "cache's own memory", k_cache=both[:, :P], k=both[:, P - 1:P + 2])
+    refuse(commit, c, ValueError, "cache's own memory", v_cache=both[:, :P], v=both[:, :3])
+    refuse(commit, c, ValueError, "v_cache is k_cache", v_cache=c["k_cache"])
+    refuse(commit, c, ValueError, "conjugates", **{x: c[x].to(torch.complex64).conj() if x == "k" else c[x].to(torch.complex64)
+                                                   for x in ("k", "v", "k_cache", "v_cache")})
     refuse(commit, c, ValueError, "multiple of 16", **{k: c[k][..., :4].contiguous() for k in ("k", "v", "k_cache", "v_cache")})
 
 
@@ -459,6 +466,16 @@ ATTEND = [
     (5, 3, [10, 900, 33, 0, 2000], 12, 1, 200, 16, "chain"),
     (40, 5, [(i * 37) % 300 for i in range(40)], 16, 4, 64, 16, "chain"),
     (30, 40, [(i * 97) % 2500 for i in range(30)], 16, 8, 64, 32, "random"),
+    # rows for 256-row workgroups: whole and cut heads, several row tiles, the head's last pieces missing
+    (2, 96, [70, 1500], 8, 2, 96, 16, "random"),
+    (1, 128, [3001], 6, 3, 72, 5, "random"),
+    (3, 128, [0, 1, 64], 16, 4, 128, 16, "random"),
+    (1, 37, [257], 32, 2, 128, 128, "chain"),
+    (2, 128, [40, 700], 2, 1, 256, 32, "random"),
+    (1, 50, [65], 8, 1, 8, 1, "flat"),
+    # 8 waves over few rows, and heads past 128 with one and more row tiles
+    (33, 2, [(i * 71) % 1200 for i in range(33)], 8, 4, 104, 16, "chain"),
+    (2, 16, [511, 513], 1, 1, 248, 64, "random"),
 ]
 
 
@@ -601,6 +618,108 @@ def test_attention_no_sequences():
     assert attend(e).shape == (0, 3, 4, 16)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,Hq,D", [(30, 12, 128), (70, 4, 136), (12, 3, 256), (2, 4, 96)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_attention_values_not_finite_by_shape(N, Hq, D, value):
+    """The same where a workgroup has 256 rows, where heads are cut, and where there are few rows."""
+    c = make_attention(9, 3, N, [200, 0, 33], Hq, 1, D, 16, BF)
+    c["v"][0, N // 2, 0, D - 1] = value
+    c["v"][1, 0, 0, 0] = value            # the root: every row
+    c["v"][2, N - 1, 0, :] = value
+    check_attention(attend(on(c)), ref_attention(**c), BF)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [4, 40])
+def test_attention_committed_values_not_finite(N):
+    """Infinity at the last committed position stays infinity: what fills its tile up does not make it NaN."""
+    c = make_attention(10, 4, N, [1, 31, 65, 640], 4, 2, 64, 16, BF)
+    for b, n in enumerate(c["lens"].tolist()):
+        page = c["block_table"][b, (n - 1) // 16].item()
+        c["v_cache"][page, (n - 1) % 16, 1, 3] = float("inf") if b % 2 else -float("inf")
+    check_attention(attend(on(c)), ref_attention(**c), BF)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [5, 40])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_attention_keys_not_finite(N, value):
+    """A key that is not finite: scores of +-infinity and NaN, in the cache and in the tree, for its rows alone."""
+    c = make_attention(11, 3, N, [100, 50, 0], 2, 2, 64, 16, BF)
+    c["k_cache"][c["block_table"][0, 2].item(), 5, 0, 7] = value
+    c["k"][1, 2, 1, 0] = value
+    c["k"][2, :, 0, 1] = value            # no other key: the row has no weights
+    ref = ref_attention(**c)
+    got = attend(on(c))
+    assert np.isnan(ref[0]).any() and np.isfinite(ref[0]).any()
+    check_attention(got, ref, BF)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [3, 40])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-3])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_scales(N, scale, dtype):
+    """Zero (the mean of the values) and negative ones, with a value that is not finite among them."""
+    c = make_attention(12, 2, N, [90, 600], 4, 2, 64, 16, dtype)
+    c["v"][1, N - 1, 0, 3] = float("inf")
+    c["scale"] = scale
+    check_attention(attend(on(c)), ref_attention(**c), dtype)
+
+
+@pytest.mark.gpu
+def test_attention_without_pages():
+    """A table without entries, a cache of one slot: the tree alone, and a length that cannot be."""
+    c = make_attention(13, 3, 4, [0, 0, 0], 2, 1, 64, 1, BF)
+    c["block_table"] = torch.zeros(3, 0, dtype=torch.int32)
+    c["lens"][2] = 1
+    check_attention(attend(on(c)), ref_attention(**c), BF)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,Hq,D", [(2, 4, 64), (24, 8, 128), (70, 8, 128)])
+def test_attention_graphs_and_streams(N, Hq, D):
+    """Sequences that are cut (work space): two captured graphs replayed in turn with eager calls between, lengths that
+    change between replays, and two streams at once."""
+    cases = [make_attention(14 + i, 2, N, [5000, 3], Hq, 2, D, 64, BF) for i in range(2)]
+    dev = [on(c) for c in cases]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for d in dev:
+            attend(d)
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, outs = [], []
+    for d in dev:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=graphs[0].pool() if graphs else None):
+            outs.append(attend(d))
+        graphs.append(g)
+    for lens in ([5000, 3], [513, 0], [1, 3]):
+        for c, d in zip(cases, dev):
+            c["lens"] = torch.tensor(lens, dtype=torch.int32)
+            d["lens"].copy_(c["lens"])
+        want = [ref_attention(**c) for c in cases]
+        for i in (0, 1, 0):
+            outs[i].fill_(7)
+            graphs[i].replay()
+            check_attention(outs[i], want[i], BF)
+            check_attention(attend(dev[1 - i]), want[1 - i], BF)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        both = []
+        for st, d in zip(streams, dev):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                both.append([attend(d) for _ in range(3)])
+        for st in streams:
+            torch.cuda.current_stream().wait_stream(st)
+        for got, w in zip(both, want):
+            for x in got:
+                check_attention(x, w, BF)
+                assert torch.equal(x, got[0])  # (the joins have one order)
+
+
 VERIFY = [
     # B, N, V, tree, drafted
     (1, 1, 1, "chain", True),
@@ -618,6 +737,10 @@ VERIFY = [
     (3, 5, 20001, "random", True),
     (2, 4, 65537, "flat", False),
     (2, 4, 65537, "flat", True),
+    (1, 3, 8192, "chain", True),
+    (1, 3, 8193, "flat", False),
+    (1, 3, 700001, "flat", True),
+    (1, 3, 700001, "flat", False),
 ]
 
 
@@ -685,6 +808,60 @@ def test_verify_edges(drafted):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [40, 300, 20000])
+def test_verify_drafts_that_take_nearly_all(V):
+    """Drafts without probabilities that hold nearly the whole row: what is left after them, parts of a sum among it, is
+    summed anew."""
+    B, N = 8, 20
+    c = make_verify(15, B, N, V, torch.float32, "flat", False)
+    g = np.random.default_rng(15)
+    rest = g.random((B, N, V)).astype(np.float32) * np.float32(2 ** -40)
+    c["target"] = torch.tensor(rest)
+    for b in range(B):
+        x = g.choice(V, N - 1, replace=False)
+        c["ids"][b, 1:] = torch.tensor(x)
+        c["target"][b, :, x] = torch.tensor(g.random(N - 1).astype(np.float32))
+        c["u"][b, 1:] = 1.0 if b % 2 else float(0.99)
+        c["u"][b, 0] = float(g.random())
+    want = ref_verify(c["parents"], c["ids"], c["target"], None, c["u"])
+    assert (want[0] == 1).any()
+    check_verify(verify(on(c)), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafted", [True, False])
+def test_verify_numbers_outside(drafted):
+    """u that is NaN, negative or not below 1: no child is kept for NaN, the next id is the first or the last with mass."""
+    c = make_verify(16, 8, 6, 3000, BF, "chain", drafted)
+    c["target"][..., -100:] = 0
+    for b, x in enumerate((float("nan"), -1.0, 1.0, 2.0, float("inf"), -float("inf"))):
+        c["u"][b] = x
+    check_verify(verify(on(c)), ref_verify(c["parents"], c["ids"], c["target"], c["draft"], c["u"]))
+
+
+@pytest.mark.gpu
+def test_verify_captured():
+    """Replays over new numbers, with eager calls between; shared rows (stride 0)."""
+    c = make_verify(17, 4, 8, 9000, torch.float32, "random")
+    d = on(c)
+    verify(d)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = verify(d)
+    gen = torch.Generator().manual_seed(1)
+    for _ in range(4):
+        c["u"] = torch.rand(4, 8, generator=gen)
+        d["u"].copy_(c["u"])
+        g.replay()
+        want = ref_verify(c["parents"], c["ids"], c["target"], c["draft"], c["u"])
+        check_verify(out, want)
+        check_verify(verify(d), want)
+    one = {**c, "target": c["target"][:1, :1].expand(4, 8, -1), "draft": c["draft"][:1, :1].expand(4, 8, -1)}
+    e = {**d, "target": d["target"][:1, :1].expand(4, 8, -1), "draft": d["draft"][:1, :1].expand(4, 8, -1)}
+    check_verify(verify(e), ref_verify(one["parents"], one["ids"], one["target"], one["draft"], one["u"]))
+
+
+@pytest.mark.gpu
 def test_verify_follows_the_target():
     """The next token is distributed as the target's row, whatever the draft: 4096 sequences of three drafts of
     the root (the same rows, own numbers), every id's share within 5 standard deviations."""
@@ -741,6 +918,23 @@ def test_commit_what_does_not_fit_is_left():
     assert torch.equal(d["k_cache"].cpu(), kc) and torch.equal(d["v_cache"].cpu(), vc)
 
 
+@pytest.mark.gpu
+def test_commit_edges():
+    """The same node twice, no pages at all, no nodes kept, many layers."""
+    c = make_commit(23, 9, 3, 5, [0, 30, 7], 1, 8, 4, BF)
+    c["n"][:] = torch.tensor([5, 0, 3])
+    c["path"][0] = torch.tensor([1, 1, 0, 4, 4])
+    kc, vc, want = ref_commit(c)
+    d = on(c)
+    assert torch.equal(commit(d).cpu(), want)
+    assert torch.equal(d["k_cache"].cpu(), kc) and torch.equal(d["v_cache"].cpu(), vc)
+    d = on({**c, "block_table": torch.zeros(3, 0, dtype=torch.int32)})
+    assert commit(d).tolist() == [-1, 30, -1]
+    assert torch.equal(d["k_cache"].cpu(), c["k_cache"]) and torch.equal(d["v_cache"].cpu(), c["v_cache"])
+    e = {k: v[:, :0] if k in ("k", "v") else v if k in ("k_cache", "v_cache") else v[:0] for k, v in on(c).items()}
+    assert commit(e).shape == (0,)
+
+
 # ---------------------------------------------------------------- the tokenizer's own path
 class _Vocabulary:
     """What BPE.id_ranges needs, without a device: 20 residue tokens and merges, 3 bins an angle."""
@@ -759,7 +953,8 @@ def test_id_ranges_follow_the_encoded_order():
     assert r.tolist() == [[0, 20], [23, 26], [26, 29], [20, 23]] and v.vocab_size == 29
     assert v.id_ranges("cpu") is v.id_ranges("cpu") and torch.equal(v.id_ranges("cpu"), torch.tensor(r))
     v._tokens = dict.fromkeys(range(25))
-    assert v.id_ranges("cpu")[0].tolist() == [0, 25]
+    old = v._id_ranges
+    assert v.id_ranges("cpu")[0].tolist() == [0, 25] and len(old) == 2  # (a graph may hold the earlier one)
     with pytest.raises(ValueError, match="29|34"):
         v.verify_draft(None, None, torch.zeros(1, 1, 12), None, None, None)
     v.res_init = False
