@@ -207,6 +207,9 @@ int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p,
   a.scale = (float)x.scale;
   a.per = plan.per;
   a.most = plan.most;
+  a.row_tiles = (int)plan.row_tiles;
+  a.by_G = page_div(a.Hq / a.Hkv), a.by_Hkv = page_div(a.Hkv), a.by_most = page_div(a.most), a.by_per = page_div(a.per),
+  a.by_RT = page_div(a.row_tiles);
   a.part = (float*)d_work;
   OnDevice on(device);
   if (!on.ok) return fail(GEOBPE_EHIP, "tree attention: device %d", device);

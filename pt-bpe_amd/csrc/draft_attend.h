@@ -22,9 +22,10 @@ struct AttendArgs {
   uint32_t kpage, kslot, vpage, vslot;
   int64_t table_stride, parents_stride;
   int32_t B, N, Hq, Hkv, D, S, P, M;  // S: page size, P: pages, M: table entries a sequence
-  PageDiv div;
+  PageDiv div;                          // S
   float scale;
-  int32_t per, most;  // tiles a part of a sequence's keys has at most, parts there are room for
+  int32_t per, most, row_tiles;         // tiles a part of a sequence's keys has at most, parts there are room for
+  PageDiv by_G, by_Hkv, by_most, by_per, by_RT;
   float* part;        // [row tile][item][part][row][D], then {max, sum} [row tile][item][part][row]
 };
 
@@ -80,10 +81,7 @@ __device__ inline uint64_t pack4(f32x4 v) {
 // negative scale turns the queries' signs.  A scale of 0 leaves a c that is too small to matter: -inf, what is not
 // there, stays -inf.
 __device__ inline float score_scale(float scale) { return fmaxf(fabsf(scale) * LOG2E, 1e-30f); }
-__device__ inline u32x4 signed_by(u32x4 q, float scale) {
-  const uint32_t s = scale < 0.f ? 0x80008000u : 0u;
-  return q ^ u32x4{s, s, s, s};
-}
+__device__ inline u32x4 negative(u32x4 q) { return q ^ u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u}; }
 // a row that has seen no key has the maximum -inf: its weights are taken from 0, and are 0
 __device__ inline float at_least(float mx) { return mx == -INFINITY ? 0.f : mx; }
 
@@ -123,21 +121,47 @@ __device__ inline bool not_finite(u32x4 v) {
 }
 
 // The tree of one sequence in LDS: anc[i] the set of nodes on the path from the root to i (i included),
-// empty when i is absent.
+// empty when i is absent.  The first wave works it out.
 struct Tree {
-  int par[DRAFT_MAX_NODES];
-  uint32_t anc[DRAFT_MAX_NODES][4];
+  int up[DRAFT_MAX_NODES];
+  __attribute__((aligned(16))) uint32_t anc[DRAFT_MAX_NODES][4];
 };
 // in two halves, so that what the caller loads meanwhile is not waited for in between
-__device__ inline int tree_parent(int N, const int32_t* parents) { return threadIdx.x < N ? parents[threadIdx.x] : 0; }
-__device__ inline void tree_paths(Tree& tr, int N, int parent) {
+struct Parents {
+  int of[2];
+};
+__device__ inline Parents tree_parents(int N, const int32_t* parents) {
   const int t = threadIdx.x;
-  if (t < N) tr.par[t] = parent;
-  __syncthreads();
-  if (t < N) {
-    uint32_t w[4];
-    draft_path(tr.par, t, w);
-    for (int k = 0; k < 4; k++) tr.anc[t][k] = w[k];
+  return {{t < 64 && t < N ? parents[t] : -2, t < 64 && t + 64 < N ? parents[t + 64] : -2}};
+}
+__device__ inline void tree_paths(Tree& tr, int N, Parents parents) {
+  const int t = threadIdx.x;
+  if (t < 64) {
+    const int nodes = N > 64 ? 2 : 1;
+    DraftNode n[2];
+    auto put = [&](int i, const DraftNode& x) {
+      tr.up[i] = x.up;
+      *(u32x4*)tr.anc[i] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+    };
+    for (int k = 0; k < 2; k++) n[k] = draft_node(t + 64 * k, parents.of[k]);
+    for (;;) {
+      for (int k = 0; k < 2; k++)
+        if (k < nodes) put(t + 64 * k, n[k]);
+      wave_order();
+      if (!__any(n[0].up >= 0 || n[1].up >= 0)) break;
+      DraftNode above[2];
+      for (int k = 0; k < 2; k++)
+        if (k < nodes && n[k].up >= 0) {
+          above[k].up = tr.up[n[k].up];
+          const u32x4 w = *(const u32x4*)tr.anc[n[k].up];
+          for (int i = 0; i < 4; i++) above[k].w[i] = w[i];
+        }
+      wave_order();
+      for (int k = 0; k < 2; k++)
+        if (k < nodes && n[k].up >= 0) draft_climb(n[k], above[k]);
+    }
+    for (int k = 0; k < 2; k++)
+      if (k < nodes && n[k].up != -1) *(u32x4*)tr.anc[t + 64 * k] = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
 }
@@ -167,8 +191,13 @@ struct Share {
 };
 __device__ inline Share share_of(const AttendArgs& a, int tiles, int part) {
   Share s;
-  const int size = (tiles + (tiles + a.per - 1) / a.per - 1) / ((tiles + a.per - 1) / a.per);
-  s.parts = (tiles + size - 1) / size;
+  int parts, left, size = tiles;
+  page_split(a.by_per, tiles + a.per - 1, parts, left);
+  s.parts = 1;
+  if (parts > 1) {
+    size = (tiles + parts - 1) / parts;
+    s.parts = (tiles + size - 1) / size;
+  }
   s.first = part * size;
   s.last = min(s.first + size, tiles);
   return s;
@@ -198,12 +227,15 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
   __shared__ Tree tr;
   __shared__ float ml[2][W][RB * 16];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l16 = lane & 15, lq = lane >> 4;
-  const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + RB * 16 - 1) / (RB * 16);
+  const int G = a.by_G.d, M = a.N * G;
   // blocks go to the 8 dies in turn: the row tiles of one part stay on one die, one after the other
   const int die = blockIdx.x & 7, j8 = blockIdx.x >> 3;
-  const int rt = j8 % RT, work = (j8 / RT) * 8 + die;
+  int rt, work, part, item, h, b;
+  page_split(a.by_RT, j8, work, rt);
+  work = work * 8 + die;
   if (work >= a.B * a.Hkv * a.most) return;
-  const int part = work % a.most, item = work / a.most, h = item % a.Hkv, b = item / a.Hkv;
+  page_split(a.by_most, work, item, part);
+  page_split(a.by_Hkv, item, b, h);
   const Span sp = span_of(a, b, ATT_TILE);
   const Share sh = share_of(a, sp.tiles, part);
   if (part >= sh.parts) return;
@@ -218,15 +250,21 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
   bool bad = sp.bad;
 
   // what does not hang on the length is loaded first
-  const int parent = tree_parent(a.N, a.parents + b * a.parents_stride);
+  const Parents parents = tree_parents(a.N, a.parents + b * a.parents_stride);
   u32x4 qf[RB][KS];
+  int node[RB];  // of the lane's rows (0 past the last row)
   for (int r = 0; r < RB; r++) {
-    const int m = (rt * RB + r) * 16 + l16, n = m / G;
-    const T* q = (const T*)a.q + b * a.qs[0] + n * a.qs[1] + (h * G + m - n * G) * a.qs[2];
+    const int m = (rt * RB + r) * 16 + l16;
+    int g;
+    page_split(a.by_G, m < M ? m : 0, node[r], g);
+    const T* q = (const T*)a.q + b * a.qs[0] + node[r] * a.qs[1] + (h * G + g) * a.qs[2];
     for (int k = 0; k < KS; k++) {
       const int d = 32 * k + 8 * lq;
       const u32x4 zero = {0, 0, 0, 0};
-      qf[r][k] = m < M && d < a.D ? signed_by(*(const u32x4*)(q + d), a.scale) : zero;
+      if (m < M && d < a.D)
+        qf[r][k] = *(const u32x4*)(q + d);
+      else
+        qf[r][k] = zero;
     }
   }
   // A tile as the lane loads it: keys l4 and 16 + l4 (past the end the last key again), pieces 4 k + p4 of them, so that
@@ -265,6 +303,12 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
            (const T*)(vc + cache_row(x.id[c], x.slot[c], a.vpage, a.vslot)));
     }
   };
+  auto fetch_nodes = [&](int tile) {
+    for (int c = 0; c < 2; c++) {
+      const int n = min((tile - sp.cache_tiles) * ATT_TILE + 16 * c + l4, a.N - 1);
+      load(c, kd + n * a.kds[1], vd + n * a.vds[1]);
+    }
+  };
   // one tile of a wave is on its way while another is worked on (with two on their way nothing got faster: 25.5 us
   // against 24.7, and 40 against 27 where the registers then hold one workgroup a CU)
   const int cached = min(last, sp.cache_tiles);
@@ -274,7 +318,10 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
     fetch();
     find(tile + W);
   }
-  tree_paths(tr, a.N, parent);
+  tree_paths(tr, a.N, parents);
+  if (a.scale < 0.f)  // (here, where the queries have to be there: nothing above waits for them)
+    for (int r = 0; r < RB; r++)
+      for (int k = 0; k < KS; k++) qf[r][k] = negative(qf[r][k]);
 
   float top[RB], sum[RB];
   f32x4 o[DB][RB];
@@ -321,12 +368,14 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
     if (!nodes && tile + W < cached) {
       fetch();
       find(tile + 2 * W);
+    } else if (!nodes && tile + W < last) {
+      fetch_nodes(tile + W);
     }
     u32x4 p[RB];
     for (int r = 0; r < RB; r++) {
       if constexpr (nodes) {
         const int m = (rt * RB + r) * 16 + l16;
-        const uint32_t set = m < M ? tr.anc[m / G][base / 32] : 0;
+        const uint32_t set = m < M ? tr.anc[node[r]][base / 32] : 0;
         for (int c = 0; c < 2; c++)
           for (int i = 0; i < 4; i++)
             if (!(set >> (16 * c + 4 * lq + i) & 1)) s[c][r][i] = -INFINITY;
@@ -377,10 +426,10 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
         for (int d = 0; d < DB; d++) *(f32x4*)(mine + 16 * d) = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int j = 0; j < ATT_TILE && base + j < a.N; j++) {
-          if (m >= M || !(tr.anc[m / G][base / 32] >> j & 1)) continue;
+          if (m >= M || !(tr.anc[node[r]][base / 32] >> j & 1)) continue;
           const T* v = vd + (base + j) * a.vds[1];
           const T* k = kd + (base + j) * a.kds[1];
-          const T* q = (const T*)a.q + b * a.qs[0] + (m / G) * a.qs[1] + (h * G + m % G) * a.qs[2];
+          const T* q = (const T*)a.q + b * a.qs[0] + node[r] * a.qs[1] + (h * G + m - node[r] * G) * a.qs[2];
           float dot = 0.f;
 #pragma unroll 1
           for (int e = 0; e < a.D; e++) dot = fmaf((float)q[e], (float)k[e], dot);
@@ -401,14 +450,11 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
     }
   };
   for (; tile < cached; tile += W) step(std::false_type(), tile * ATT_TILE);
-  for (; tile < last; tile += W) {
-    const int base = (tile - sp.cache_tiles) * ATT_TILE;
-    for (int c = 0; c < 2; c++) {
-      const int n = min(base + 16 * c + l4, a.N - 1);
-      load(c, kd + n * a.kds[1], vd + n * a.vds[1]);
-    }
-    step(std::true_type(), base);
+  if (tile < last) {  // the nodes (at most 32, as there are no more rows): one tile, of one wave
+    if (tile < first + W) fetch_nodes(tile);  // (else loaded in its last step)
+    step(std::true_type(), (tile - sp.cache_tiles) * ATT_TILE);
   }
+
 
   // the waves' sums joined: maxima first, then 16 rows at a time through LDS
   for (int r = 0; r < RB; r++) {
@@ -437,17 +483,18 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
         total += f * ml[1][w][r * 16 + row];
         acc += f * *(const f32x4*)((const float*)(lds + w * AREA) + row * (DP + 4) + d);
       }
-      const int n = m / G;
+      int n, g;
+      page_split(a.by_G, m, n, g);
       const bool here = tr.anc[n][n / 32] >> (n % 32) & 1;
       if (sh.parts == 1) {
-        T* out = (T*)a.out + (((int64_t)b * a.N + n) * a.Hq + h * G + m - n * G) * a.D + d;
+        T* out = (T*)a.out + (((int64_t)b * a.N + n) * a.Hq + h * G + g) * a.D + d;
         *(uint64_t*)out = here ? pack4<T>(acc * (1.f / total)) : 0;
       } else {
         const int64_t at = part_row(a, rt, item, part, RB * 16, r * 16 + row);
         const f32x4 none = {0.f, 0.f, 0.f, 0.f};  // an absent row's parts: a sum of 0
         *(f32x4*)(a.part + at * a.D + d) = here ? acc : none;
         if (d == 0) {
-          float* p = part_sums(a, RT, RB * 16) + 2 * at;
+          float* p = part_sums(a, a.row_tiles, RB * 16) + 2 * at;
           p[0] = here ? mx : -INFINITY;
           p[1] = here ? total : 0.f;
         }
@@ -526,15 +573,20 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, hh = lane >> 5;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   const float scale = score_scale(a.scale);
-  const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + ROWS - 1) / ROWS;
+  const int G = a.by_G.d, M = a.N * G;
   const int die = blockIdx.x & 7, j8 = blockIdx.x >> 3;
-  const int rt = uni(j8 % RT), work = uni((j8 / RT) * 8 + die);
+  int rt, work, part, item, h, b;
+  page_split(a.by_RT, j8, work, rt);
+  work = work * 8 + die;
   if (work >= a.B * a.Hkv * a.most) return;
-  const int part = uni(work % a.most), item = uni(work / a.most), h = uni(item % a.Hkv), b = uni(item / a.Hkv);
+  page_split(a.by_most, work, item, part);
+  page_split(a.by_Hkv, item, b, h);
   const Span sp = span_of(a, b, WIDE_TILE);
   const Share sh = share_of(a, sp.tiles, part);
   if (part >= sh.parts) return;
-  const int m = rt * ROWS + wave * 32 + l32, node = m / G;
+  const int m = rt * ROWS + wave * 32 + l32;
+  int node, head;  // (of row 0 past the last row)
+  page_split(a.by_G, m < M ? m : 0, node, head);
   const bool rows = rt * ROWS + uni(wave) * 32 < M;  // (the wave has any)
 
   // where this lane's operands lie in a tile: K's piece 2 k + hh of row l32, V's four keys of 16 channels
@@ -546,6 +598,17 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
     const int row = 4 * hh + (lane >> 2 & 3), col = 32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
     voff[d] = lds_at + VBUF + (row * CH + ((col / 8) ^ vswz(row))) * 16 + (col & 4) * 2;
   }
+  // a wave's 32 rows of the queries and of the result lie in the tiles' place, as K's rows do, before and after them; lane l
+  // moves piece l % CH of the rows l / CH + 64 / CH i (in the operands' own order, 32 bytes of a row at a time, the queries
+  // took 2 us longer and the result 2.5)
+  const uint32_t own = wave * 32 * CH * 16;
+  auto row_of = [&](int i, int64_t* at, const int64_t* st) {  // the row's place by its node's and head's strides; false: no row
+    const int x = rt * ROWS + wave * 32 + lane / CH + 64 / CH * i;
+    int n, g;
+    page_split(a.by_G, x < M ? x : 0, n, g);
+    *at = n * st[0] + (h * G + g) * st[1];
+    return x < M;
+  };
   // thread t moves piece t % CH (as it lies in LDS) of the rows t / CH + RPI i
   const int prow = t / CH, pc = t % CH;
 
@@ -558,6 +621,19 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
     for (int d = 0; d < DB; d++)
       for (int i = 0; i < 16; i++) o[d][i] = 0.f;
     u32x4 qf[KSTEPS];
+    // the nodes' keys and values, in the same way as the cache's
+    int nkb = 0, nvb = 0;  // the buffers they are in
+    const T* kd = (const T*)a.kd + b * a.kds[0] + h * a.kds[2];
+    const T* vd = (const T*)a.vd + b * a.vds[0] + h * a.vds[2];
+    auto stage_nodes = [&](int tile) {
+      for (int i = 0; i < PER; i++) {
+        const int row = prow + RPI * i, n = min((tile - uni(sp.cache_tiles)) * WIDE_TILE + row, a.N - 1);
+        const int ck = (pc ^ kswz(row)) * 8, cv = (pc ^ vswz(row)) * 8;
+        const uint32_t to = lds_at + wave * 1024 + i * BLOCK * 16;
+        to_lds(FULL || ck < a.D ? (const void*)(kd + n * a.kds[1] + ck) : att_zero, to + nkb * TILE_BYTES);
+        to_lds(FULL || cv < a.D ? (const void*)(vd + n * a.vds[1] + cv) : att_zero, to + VBUF + nvb * TILE_BYTES);
+      }
+    };
 
     auto scores = [&](f32x16* s, uint32_t buf) {
       for (int c = 0; c < 2; c++) {
@@ -603,15 +679,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
     {
       const int len = uni(sp.len);
       if (t == 0) odd_ = 0;
-      const int parent = tree_parent(a.N, a.parents + b * a.parents_stride);  // (what does not hang on the length first)
-      const T* q = (const T*)a.q + b * a.qs[0] + node * a.qs[1] + (h * G + m - node * G) * a.qs[2];
-      for (int k = 0; k < KSTEPS; k++) {
-        const int d = 16 * k + 8 * hh;
-        if (m < M && d < a.D)
-          qf[k] = signed_by(*(const u32x4*)(q + d), a.scale);
-        else
-          qf[k] = u32x4{0, 0, 0, 0};
-      }
+      const Parents parents = tree_parents(a.N, a.parents + b * a.parents_stride);
       const Pages pages = {a.table + b * a.table_stride, a.div, a.P, a.M};
       const char* kc = (const char*)((const T*)a.kc + h * a.khead);
       const char* vc = (const char*)((const T*)a.vc + h * a.vhead);
@@ -637,6 +705,13 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
           to_lds(FULL || c < a.D ? (const void*)p : att_zero, to + i * BLOCK * 16);
         }
       };
+      if (rows)
+        for (int i = 0; i < CH / 2; i++) {
+          const int row = lane / CH + 64 / CH * i, c = ((lane % CH) ^ kswz(row)) * 8;
+          int64_t at;
+          const bool in = row_of(i, &at, a.qs + 1) && (FULL || c < a.D);
+          to_lds(in ? (const void*)((const T*)a.q + b * a.qs[0] + at + c) : att_zero, lds_at + own + i * 1024);
+        }
       const int n_cached = cached - tile;  // (of this part; at most 0 when it has the nodes alone)
       if (n_cached > 0) {
         find(first + wave);
@@ -644,13 +719,22 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
           locate(wave);
           find(first + wave + 4);
         }
-        __syncthreads();
-        wait_loads();
+      }
+      wait_loads();
+      if (rows) {
+        for (int k = 0; k < KSTEPS; k++) qf[k] = lds_read<u32x4>(koff[k] + own, 0);
+        if (a.scale < 0.f)
+          for (int k = 0; k < KSTEPS; k++) qf[k] = negative(qf[k]);
+      }
+      __syncthreads();
+      if (n_cached <= 0) {
+        stage_nodes(tile);
+      } else {
         stage(0, 0, 0);
         stage(0, 1, 0);
         if (n_cached > 1) stage(1, 0, 1);
       }
-      tree_paths(tr, a.N, parent);
+      tree_paths(tr, a.N, parents);
 
       // The cache's tiles: a tile's scores are worked out while the weights of the one before it are, in the matrix
       // unit and beside it.  So K comes two tiles ahead and V one.
@@ -745,6 +829,10 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
           s[1] = n[1];
         }
         arrive(t, t & 1);
+        if (cached < last) {
+          nvb = t & 1 ^ 1;
+          stage_nodes(cached);
+        }
         if (rows) {
           u32x4 p[4];
           weigh(s, p);
@@ -755,44 +843,46 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
     }
 
     // the tree's own keys, one tile after the other
-    for (; tile < last; tile++) {
+    while (tile < last) {
       const int base = (tile - uni(sp.cache_tiles)) * WIDE_TILE;
-      const T* kd = (const T*)a.kd + b * a.kds[0] + h * a.kds[2];
-      const T* vd = (const T*)a.vd + b * a.vds[0] + h * a.vds[2];
-      __syncthreads();
-      // through registers: a value that is not finite would reach every row as 0 times itself; it goes in as 0 and is
-      // added on its own path
+      wait_loads();
+      // a value that is not finite would reach every row as 0 times itself: it becomes 0 and is added on its own path
       for (int i = 0; i < PER; i++) {
-        const int row = prow + RPI * i, n = min(base + row, a.N - 1);
-        const int ck = (pc ^ kswz(row)) * 8, cv = (pc ^ vswz(row)) * 8;
-        const u32x4 k = keep_if(ck < a.D, *(const u32x4*)(kd + n * a.kds[1] + (ck < a.D ? ck : 0)));
-        u32x4 v = keep_if(cv < a.D, *(const u32x4*)(vd + n * a.vds[1] + (cv < a.D ? cv : 0)));
-        if (not_finite<T>(v)) odd_ = 1;
-        v = keep_if(!not_finite<T>(v), v);
-        *(u32x4*)(lds + (t + BLOCK * i) * 16) = k;
-        *(u32x4*)(lds + VBUF + (t + BLOCK * i) * 16) = v;
+        u32x4* at = (u32x4*)(lds + VBUF + nvb * TILE_BYTES + (t + BLOCK * i) * 16);
+        if (not_finite<T>(*at)) {
+          *at = u32x4{0, 0, 0, 0};
+          odd_ = 1;
+        }
       }
       __syncthreads();
-      if (!rows) continue;
+      const int kb = nkb, vb = nvb;
+      const bool more = ++tile < last, odd = odd_;
+      if (more && !odd) {  // (else the other buffers are needed below)
+        nkb ^= 1;
+        nvb ^= 1;
+        stage_nodes(tile);
+      }
       f32x16 s[2];
       u32x4 p[4];
-      scores(s, 0);
-      for (int c = 0; c < 2; c++) {
-        const uint32_t set = m < M ? tr.anc[node][base / 32 + c] : 0;
-        for (int i = 0; i < 16; i++)
-          if (!(set >> (8 * (i / 4) + 4 * hh + i % 4) & 1)) s[c][i] = -INFINITY;
+      if (rows) {
+        scores(s, kb * TILE_BYTES);
+        for (int c = 0; c < 2; c++) {
+          const uint32_t set = m < M ? tr.anc[node][base / 32 + c] : 0;
+          for (int i = 0; i < 16; i++)
+            if (!(set >> (8 * (i / 4) + 4 * hh + i % 4) & 1)) s[c][i] = -INFINITY;
+        }
+        follow(s);
+        weigh(s, p);
+        product(p, vb * TILE_BYTES);
       }
-      follow(s);
-      weigh(s, p);
-      product(p, 0);
-      if (!odd_) continue;
+      if (!odd) continue;
       // the sums of what went in as 0 (the finite values of its pieces with their weights), some of the channels at a time,
       // in the LDS that the tile does not use
       constexpr int TURNS = W / 2, DT = DP / TURNS;
 #pragma unroll
-      for (int turn = 0; turn < TURNS; turn++) {
+      for (int turn = 0; turn < TURNS && rows; turn++) {
         const int slice = wave * 32 + l32, d0 = turn * DT;
-        float* mine = (float*)(lds + (slice < ROWS / 2 ? TILE_BYTES : VBUF + TILE_BYTES)) + slice % (ROWS / 2) * DT;
+        float* mine = (float*)(lds + (slice < ROWS / 2 ? (kb ^ 1) * TILE_BYTES : VBUF + (vb ^ 1) * TILE_BYTES)) + slice % (ROWS / 2) * DT;
 #pragma unroll 1
         for (int d = 4 * hh; d < DT; d += 8) *(f32x4*)(mine + d) = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
@@ -800,7 +890,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
           if (m >= M || !(tr.anc[node][(base + j) / 32] >> (j % 32) & 1)) continue;
           const T* v = vd + (base + j) * a.vds[1];
           const T* k = kd + (base + j) * a.kds[1];
-          const T* q = (const T*)a.q + b * a.qs[0] + node * a.qs[1] + (h * G + m - node * G) * a.qs[2];
+          const T* q = (const T*)a.q + b * a.qs[0] + node * a.qs[1] + (h * G + head) * a.qs[2];
           float dot = 0.f;
 #pragma unroll 1
           for (int e = 0; e < a.D; e++) dot = fmaf((float)q[e], (float)k[e], dot);
@@ -825,6 +915,8 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
           }
         wave_order();
       }
+      __syncthreads();
+      if (more) stage_nodes(tile);
     }
 
     sum += __shfl_xor(sum, 32);
@@ -833,9 +925,8 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
       const int64_t at = part_row(a, rt, item, part, ROWS, wave * 32 + l32);
       const bool here = tr.anc[node][node / 32] >> (node % 32) & 1;
       const float f = 1.f / sum;
-      T* out = (T*)a.out + (((int64_t)b * a.N + node) * a.Hq + h * G + m - node * G) * a.D;
       if (sh.parts > 1 && hh == 0) {
-        float* ml = part_sums(a, RT, ROWS) + 2 * at;
+        float* ml = part_sums(a, a.row_tiles, ROWS) + 2 * at;
         ml[0] = here ? top : -INFINITY;
         ml[1] = here ? sum : 0.f;
       }
@@ -847,8 +938,19 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
           if (sh.parts > 1)  // (an absent row's parts: a sum of 0)
             *(f32x4*)(a.part + at * a.D + x) = here ? y : none;
           else
-            *(uint64_t*)(out + x) = here ? pack4<T>(y * f) : 0;
+            *(uint64_t*)(lds + own + (l32 * CH + ((4 * d + i) ^ kswz(l32))) * 16 + 8 * hh) = here ? pack4<T>(y * f) : 0;
         }
+    }
+    if (sh.parts == 1 && rows) {
+      wave_order();
+      const int64_t st[2] = {(int64_t)a.Hq * a.D, a.D};
+      for (int i = 0; i < CH / 2; i++) {
+        const int c = lane % CH, row = lane / CH + 64 / CH * i;
+        int64_t at;
+        if (row_of(i, &at, st) && (FULL || c * 8 < a.D))
+          *(u32x4*)((T*)a.out + (int64_t)b * a.N * st[0] + at + c * 8) =
+              *(const u32x4*)(lds + own + (row * CH + (c ^ kswz(row))) * 16);
+      }
     }
   }
 }
@@ -859,7 +961,7 @@ template <typename T, int BY, int J>
 __global__ __launch_bounds__(ATT_BLOCK) void k_attend_join(AttendArgs a, int rows, int tile) {
   __shared__ f32x4 acc_[BY > 1 ? ATT_BLOCK : 1];
   __shared__ float ml_[2][BY > 1 ? ATT_BLOCK : 1];
-  const int G = a.Hq / a.Hkv, M = a.N * G, RT = (M + rows - 1) / rows, t = threadIdx.x;
+  const int G = a.by_G.d, M = a.N * G, t = threadIdx.x;
   const int q = a.D / 4, each = ATT_BLOCK / (q * BY);  // rows a workgroup
   const int r = t / (q * BY), by = t / q % BY, d = t % q * 4;
   const uint32_t x = blockIdx.x * each + r;  // (the host keeps the rows below 2^31)
@@ -868,7 +970,7 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend_join(AttendArgs a, int row
   const int parts = on ? share_of(a, span_of(a, b, tile).tiles, 0).parts : 1;
   const float scale = score_scale(a.scale);
   const int64_t base = part_row(a, m / rows, bh, 0, rows, m % rows);
-  const float* ml = part_sums(a, RT, rows);
+  const float* ml = part_sums(a, a.row_tiles, rows);
   float mx = -INFINITY, total = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   auto add = [&](float m2, float l2, f32x4 v) {
