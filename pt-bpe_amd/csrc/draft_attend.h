@@ -111,6 +111,12 @@ __device__ inline u32x4 keep_if(bool in, u32x4 y) {
   return y;
 }
 
+// s where the set's bit is 1, else -infinity
+__device__ inline float if_bit(uint32_t set, int bit, float s) {
+  const uint32_t in = (int32_t)(set << (31 - bit)) >> 31;
+  return __uint_as_float((__float_as_uint(s) & in) | (0xff800000u & ~in));
+}
+
 // exponent all ones in any of the eight halves
 template <typename T>
 __device__ inline bool not_finite(u32x4 v) {
@@ -375,10 +381,9 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
     for (int r = 0; r < RB; r++) {
       if constexpr (nodes) {
         const int m = (rt * RB + r) * 16 + l16;
-        const uint32_t set = m < M ? tr.anc[node[r]][base / 32] : 0;
+        const uint32_t set = m < M ? tr.anc[node[r]][base / 32] >> (4 * lq) : 0;
         for (int c = 0; c < 2; c++)
-          for (int i = 0; i < 4; i++)
-            if (!(set >> (16 * c + 4 * lq + i) & 1)) s[c][r][i] = -INFINITY;
+          for (int i = 0; i < 4; i++) s[c][r][i] = if_bit(set, 16 * c + i, s[c][r][i]);
       } else if (base + ATT_TILE > sp.len) {
         for (int c = 0; c < 2; c++)
           for (int i = 0; i < 4; i++)
@@ -602,12 +607,21 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
   // moves piece l % CH of the rows l / CH + 64 / CH i (in the operands' own order, 32 bytes of a row at a time, the queries
   // took 2 us longer and the result 2.5)
   const uint32_t own = wave * 32 * CH * 16;
-  auto row_of = [&](int i, int64_t* at, const int64_t* st) {  // the row's place by its node's and head's strides; false: no row
-    const int x = rt * ROWS + wave * 32 + lane / CH + 64 / CH * i;
-    int n, g;
-    page_split(a.by_G, x < M ? x : 0, n, g);
-    *at = n * st[0] + (h * G + g) * st[1];
-    return x < M;
+  auto walk = [&](const T* p, int64_t by_node, int64_t by_head, auto&& row) {
+    const int step = 64 / CH, x = rt * ROWS + wave * 32 + lane / CH;
+    int n, g, dn, dg;
+    page_split(a.by_G, x, n, g);
+    page_split(a.by_G, step, dn, dg);
+    p += n * by_node + (h * G + g) * by_head;
+    for (int i = 0; i < CH / 2; i++) {  // (a row's place from the last one's: 64-bit products are the dearest instructions here)
+      row(i, p, x + step * i < M);
+      p += dn * by_node + dg * by_head;
+      g += dg;
+      if (g >= G) {
+        g -= G;
+        p += by_node - G * by_head;
+      }
+    }
   };
   // thread t moves piece t % CH (as it lies in LDS) of the rows t / CH + RPI i
   const int prow = t / CH, pc = t % CH;
@@ -706,12 +720,10 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
         }
       };
       if (rows)
-        for (int i = 0; i < CH / 2; i++) {
-          const int row = lane / CH + 64 / CH * i, c = ((lane % CH) ^ kswz(row)) * 8;
-          int64_t at;
-          const bool in = row_of(i, &at, a.qs + 1) && (FULL || c < a.D);
-          to_lds(in ? (const void*)((const T*)a.q + b * a.qs[0] + at + c) : att_zero, lds_at + own + i * 1024);
-        }
+        walk((const T*)a.q + b * a.qs[0], a.qs[1], a.qs[2], [&](int i, const T* p, bool in) {
+          const int c = ((lane % CH) ^ kswz(lane / CH + 64 / CH * i)) * 8;
+          to_lds(in && (FULL || c < a.D) ? (const void*)(p + c) : att_zero, lds_at + own + i * 1024);
+        });
       const int n_cached = cached - tile;  // (of this part; at most 0 when it has the nodes alone)
       if (n_cached > 0) {
         find(first + wave);
@@ -867,9 +879,8 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
       if (rows) {
         scores(s, kb * TILE_BYTES);
         for (int c = 0; c < 2; c++) {
-          const uint32_t set = m < M ? tr.anc[node][base / 32 + c] : 0;
-          for (int i = 0; i < 16; i++)
-            if (!(set >> (8 * (i / 4) + 4 * hh + i % 4) & 1)) s[c][i] = -INFINITY;
+          const uint32_t set = m < M ? tr.anc[node][base / 32 + c] >> (4 * hh) : 0;
+          for (int i = 0; i < 16; i++) s[c][i] = if_bit(set, 8 * (i / 4) + i % 4, s[c][i]);
         }
         follow(s);
         weigh(s, p);
@@ -943,14 +954,12 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
     }
     if (sh.parts == 1 && rows) {
       wave_order();
-      const int64_t st[2] = {(int64_t)a.Hq * a.D, a.D};
-      for (int i = 0; i < CH / 2; i++) {
+      const int64_t line = (int64_t)a.Hq * a.D;
+      walk((const T*)a.out + (int64_t)b * a.N * line, line, a.D, [&](int i, const T* p, bool in) {
         const int c = lane % CH, row = lane / CH + 64 / CH * i;
-        int64_t at;
-        if (row_of(i, &at, st) && (FULL || c * 8 < a.D))
-          *(u32x4*)((T*)a.out + (int64_t)b * a.N * st[0] + at + c * 8) =
-              *(const u32x4*)(lds + own + (row * CH + (c ^ kswz(row))) * 16);
-      }
+        if (in && (FULL || c * 8 < a.D))
+          *(u32x4*)(const_cast<T*>(p) + c * 8) = *(const u32x4*)(lds + own + (row * CH + (c ^ kswz(row))) * 16);
+      });
     }
   }
 }
