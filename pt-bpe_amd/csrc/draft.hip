@@ -60,16 +60,26 @@ AttendPlan attend_plan(const geobpe_attend_args& x) {
   const int64_t M = x.nodes * (x.heads / x.kv_heads);
   p.wide = M > (x.head_dim > 128 ? 16 : 32);
   p.rb = M <= 16 ? 1 : 2;
-  p.rows = p.wide ? 32 * (M > 128 && x.head_dim > 64 && x.head_dim <= 128 ? 8 : 4) : 16 * p.rb;
   p.tile = p.wide ? WIDE_TILE : ATT_TILE;
-  p.row_tiles = (M + p.rows - 1) / p.rows;
   const int64_t tiles = (x.max_pages * x.page_size + p.tile - 1) / p.tile + (x.nodes + p.tile - 1) / p.tile;
   const int64_t items = x.seqs * x.kv_heads;
+  // Where the tiles are many: 256 rows share one where there are more than 128 and heads of 128 (32 sequences x 8 heads of
+  // 256 rows over 16k: 508 us instead of 548), 64 where there are no more and the heads are narrow, so that no wave is
+  // idle (40 x 8 heads of 48 rows over 9k: 102 us instead of 115; with heads of 64, which wait for memory, 122 instead of
+  // 114).  Where they are few 128 make more workgroups (2 heads of 432 rows over 960: 18 us instead of 22; 16 heads of 40
+  // rows over 3k: 14.1 instead of 16.0).
+  const bool many = items * ((M + 255) / 256) * tiles >= WIDE_MANY;
+  p.rows = !p.wide                                                            ? 16 * p.rb
+           : many && M > 128 && x.head_dim > 96 && x.head_dim <= 128 ? 256
+           : many && M <= 64 && x.head_dim <= 32                     ? 64
+                                                                     : 128;
+  p.row_tiles = (M + p.rows - 1) / p.rows;
   // eight waves where that fills the card without cutting the sequences (64 sequences x 4 heads: 26 us instead of 25 + 10
   // for the join); four where they are cut anyway, and more finely then (7 x 12 heads: 27 us instead of 40)
   p.waves = p.wide ? p.rows / 32 : x.head_dim <= 128 && items * p.row_tiles >= 128 && items * p.row_tiles <= 256 ? 8 : 4;
   const int64_t want = ATT_WANT * 4 / p.waves, even = (items * p.row_tiles * tiles + want - 1) / want;
-  p.per = (int)(even > tiles ? tiles : even > ATT_LEAST ? even : ATT_LEAST);
+  const int least = p.wide ? WIDE_LEAST : ATT_LEAST;
+  p.per = (int)(even > tiles ? tiles : even > least ? even : least);
   p.most = (int)((tiles + p.per - 1) / p.per);
   p.blocks = (items * p.most + 7) / 8 * 8 * p.row_tiles;
   p.bytes = p.most > 1 ? items * p.row_tiles * p.most * p.rows * (x.head_dim + 2) * 4 : 0;
@@ -110,7 +120,13 @@ template <typename T>
 void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)p.blocks), block(64 * p.waves);
   if (p.wide) {
-    if (a.D == 64)
+    if (p.waves == 2)
+      hipLaunchKernelGGL((k_attend_wide<T, 32, false, 2>), grid, block, 0, s, a);
+    else if (a.D <= 32)
+      hipLaunchKernelGGL((k_attend_wide<T, 32, false, 4>), grid, block, 0, s, a);
+    else if (a.D > 64 && a.D <= 96)
+      hipLaunchKernelGGL((k_attend_wide<T, 96, false, 4>), grid, block, 0, s, a);
+    else if (a.D == 64)
       hipLaunchKernelGGL((k_attend_wide<T, 64, true, 4>), grid, block, 0, s, a);
     else if (a.D < 64)
       hipLaunchKernelGGL((k_attend_wide<T, 64, false, 4>), grid, block, 0, s, a);

@@ -509,15 +509,38 @@ __global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 
 }
 
 // ---- many rows -------------------------------------------------------------------------------
-// Above 32 rows a kv head the keys are shared: a workgroup has 128 or 256 rows, 32 a wave, and its waves read the same
-// tiles of 64 keys from LDS.  The cache's rows go there directly, the next tile's while this one's products run.
+// Above 32 rows a kv head the keys are shared: a workgroup has 64 to 256 rows, 32 a wave, and its waves read the same
+// tiles of 64 keys from LDS.  Rows go there directly, the next tile's while this one's products run.
 // S^T = K Q^T and O^T = V^T P^T in the 32x32x16 instruction, in the same way as above: row = lane % 32, and a
 // lane's weights of four keys in a row are the second product's operand.
 //
-// In LDS a row's 16-byte pieces are permuted so that the operands' reads spread over the banks: K's piece c of
-// row r lies at c ^ (r & 7) (eight rows, one piece each), V's at c ^ 4 (r & 3) (four rows, 64 bytes each; rows of
-// 128 bytes: c ^ 4 (r / 2 & 1)).
-constexpr int WIDE_TILE = 64;
+// In LDS a row's 16-byte pieces are permuted so that the operands' reads spread over the banks: eight rows' piece of K in
+// different ones (piece c of row r lies at c ^ (r & 7), in rows of 64 bytes at c ^ (r / 4 & 1), in those of 192, whose
+// starts are in four places already, at (c + (r / 4 & 1)) % 12), four rows' 64 bytes of V too (c ^ 4 (r & 3); rows of 128
+// bytes: c ^ 4 (r / 2 & 1); rows of 64 and 192 as they are).
+template <int CH>
+__device__ inline int key_slot(int row, int c) {  // where piece c of a row of CH lies
+  if constexpr (CH == 12) {
+    const int x = c + (row >> 2 & 1);
+    return x < 12 ? x : x - 12;
+  }
+  return c ^ (CH == 4 ? row >> 2 & 1 : row & 7);
+}
+template <int CH>
+__device__ inline int key_piece(int row, int at) {  // the piece that lies there
+  if constexpr (CH == 12) {
+    const int x = at - (row >> 2 & 1);
+    return x < 0 ? x + 12 : x;
+  }
+  return key_slot<CH>(row, at);
+}
+template <int CH>
+__device__ inline int value_slot(int row, int c) {  // (its own inverse)
+  return c ^ (CH >= 16 ? (row & 3) << 2 : CH == 8 ? (row >> 1 & 1) << 2 : 0);
+}
+// A part has at least 4 tiles (2 heads of 432 rows over 960 positions, at least 16 / 8 / 4 / 2 tiles: 36 / 22 / 18 / 15.5 us;
+// with 2 those over 64 took 13.2 instead of 11.0 for the join).  `Many` tiles: eight for every CU.
+constexpr int WIDE_TILE = 64, WIDE_LEAST = 4, WIDE_MANY = 2048;
 constexpr float SLACK = 8.f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -565,12 +588,13 @@ __device__ inline void wait_loads() {
 __device__ const u32x4 att_zero[32] = {};
 
 template <typename T, int DP, bool FULL, int W>
-__global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(AttendArgs a) {
+__global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_attend_wide(AttendArgs a) {
   constexpr int BLOCK = 64 * W, ROWS = 32 * W;
   constexpr int CH = DP / 8, KSTEPS = DP / 16, DB = DP / 32;
   constexpr int TILE_BYTES = WIDE_TILE * DP * 2, PER = WIDE_TILE * CH / BLOCK;  // pieces a thread moves
-  constexpr int RPI = BLOCK / CH;                                               // rows between them
+  static_assert(WIDE_TILE * CH % BLOCK == 0, "");
   constexpr uint32_t VBUF = 2 * TILE_BYTES;
+  constexpr int TURN = W < 4 ? W : 4;  // waves that take turns at working out places
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];  // K of two tiles, V of two
   __shared__ uint64_t offs[4][2][WIDE_TILE];                         // the rows' places in the cache: tile % 4, K or V
   __shared__ Tree tr;
@@ -595,36 +619,45 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
   const bool rows = rt * ROWS + uni(wave) * 32 < M;  // (the wave has any)
 
   // where this lane's operands lie in a tile: K's piece 2 k + hh of row l32, V's four keys of 16 channels
-  auto kswz = [](int row) { return row & 7 & (CH - 1); };
-  auto vswz = [](int row) { return CH >= 16 ? (row & 3) << 2 : CH == 8 ? (row >> 1 & 1) << 2 : 0; };
   uint32_t koff[KSTEPS], voff[DB];
-  for (int k = 0; k < KSTEPS; k++) koff[k] = lds_at + (l32 * CH + ((2 * k + hh) ^ kswz(l32))) * 16;
+  for (int k = 0; k < KSTEPS; k++) koff[k] = lds_at + (l32 * CH + key_slot<CH>(l32, 2 * k + hh)) * 16;
   for (int d = 0; d < DB; d++) {
     const int row = 4 * hh + (lane >> 2 & 3), col = 32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-    voff[d] = lds_at + VBUF + (row * CH + ((col / 8) ^ vswz(row))) * 16 + (col & 4) * 2;
+    voff[d] = lds_at + VBUF + (row * CH + value_slot<CH>(row, col / 8)) * 16 + (col & 4) * 2;
   }
-  // a wave's 32 rows of the queries and of the result lie in the tiles' place, as K's rows do, before and after them; lane l
-  // moves piece l % CH of the rows l / CH + 64 / CH i (in the operands' own order, 32 bytes of a row at a time, the queries
-  // took 2 us longer and the result 2.5)
+  // A wave's 32 rows of the queries and of the result lie in the tiles' place, as K's rows do, before and after them; the
+  // lanes move pieces that lie in a row (in the operands' own order, 32 bytes of a row at a time, the queries took 2 us
+  // longer and the result 2.5).
   const uint32_t own = wave * 32 * CH * 16;
-  auto walk = [&](const T* p, int64_t by_node, int64_t by_head, auto&& row) {
-    const int step = 64 / CH, x = rt * ROWS + wave * 32 + lane / CH;
-    int n, g, dn, dg;
-    page_split(a.by_G, x, n, g);
-    page_split(a.by_G, step, dn, dg);
-    p += n * by_node + (h * G + g) * by_head;
-    for (int i = 0; i < CH / 2; i++) {  // (a row's place from the last one's: 64-bit products are the dearest instructions here)
-      row(i, p, x + step * i < M);
-      p += dn * by_node + dg * by_head;
-      g += dg;
-      if (g >= G) {
-        g -= G;
-        p += by_node - G * by_head;
+  auto walk = [&](const T* p, int64_t by_node, int64_t by_head, auto&& piece) {
+    const int x = rt * ROWS + wave * 32;
+    int n, g;
+    if constexpr (CH == 12) {
+      for (int i = 0; i < CH / 2; i++) {
+        const int row = (lane + 64 * i) / CH;
+        page_split(a.by_G, x + row, n, g);
+        piece(i, row, lane + 64 * i - row * CH, p + (n * by_node + (h * G + g) * by_head), x + row < M);
+      }
+    } else {  // a row's place from the last one's: 64-bit products are the dearest instructions here
+      const int step = 64 / CH, row = lane / CH;
+      int dn, dg;
+      page_split(a.by_G, x + row, n, g);
+      page_split(a.by_G, step, dn, dg);
+      p += n * by_node + (h * G + g) * by_head;
+      for (int i = 0; i < CH / 2; i++) {
+        piece(i, row + step * i, lane % CH, p, x + row + step * i < M);
+        p += dn * by_node + dg * by_head;
+        g += dg;
+        if (g >= G) {
+          g -= G;
+          p += by_node - G * by_head;
+        }
       }
     }
   };
-  // thread t moves piece t % CH (as it lies in LDS) of the rows t / CH + RPI i
-  const int prow = t / CH, pc = t % CH;
+  // the pieces of a tile that thread t moves: at pc(i), as it lies in LDS, of row prow(i)
+  auto prow = [&](int i) { return CH == 12 ? (t + BLOCK * i) / CH : t / CH + BLOCK / CH * i; };
+  auto pc = [&](int i) { return CH == 12 ? (t + BLOCK * i) % CH : t % CH; };
 
   {
     const int first = uni(sh.first), last = uni(sh.last), cached = min(last, uni(sp.cache_tiles));
@@ -641,8 +674,8 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
     const T* vd = (const T*)a.vd + b * a.vds[0] + h * a.vds[2];
     auto stage_nodes = [&](int tile) {
       for (int i = 0; i < PER; i++) {
-        const int row = prow + RPI * i, n = min((tile - uni(sp.cache_tiles)) * WIDE_TILE + row, a.N - 1);
-        const int ck = (pc ^ kswz(row)) * 8, cv = (pc ^ vswz(row)) * 8;
+        const int row = prow(i), n = min((tile - uni(sp.cache_tiles)) * WIDE_TILE + row, a.N - 1);
+        const int ck = key_piece<CH>(row, pc(i)) * 8, cv = value_slot<CH>(row, pc(i)) * 8;
         const uint32_t to = lds_at + wave * 1024 + i * BLOCK * 16;
         to_lds(FULL || ck < a.D ? (const void*)(kd + n * a.kds[1] + ck) : att_zero, to + nkb * TILE_BYTES);
         to_lds(FULL || cv < a.D ? (const void*)(vd + n * a.vds[1] + cv) : att_zero, to + VBUF + nvb * TILE_BYTES);
@@ -698,7 +731,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
       const char* kc = (const char*)((const T*)a.kc + h * a.khead);
       const char* vc = (const char*)((const T*)a.vc + h * a.vhead);
       // A row's place is worked out once, by the lanes of one wave (the waves take turns), and goes to the others through
-      // LDS; its table entry is loaded four tiles before that, and looked at only then: nothing waits for it.
+      // LDS; its table entry is loaded TURN tiles before that, and looked at only then: nothing waits for it.
       int entry = 0, slot = 0;
       auto find = [&](int tile) { entry = page_entry(pages, min(tile * WIDE_TILE + lane, len - 1), slot); };
       auto locate = [&](int tile) {
@@ -714,22 +747,22 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
       auto stage = [&](int t, int kv, int buf) {
         const uint32_t to = lds_at + kv * VBUF + buf * TILE_BYTES + wave * 1024;  // the wave's 64 pieces in a row
         for (int i = 0; i < PER; i++) {
-          const int row = prow + RPI * i, c = (pc ^ (kv ? vswz(row) : kswz(row))) * 8;
+          const int row = prow(i), c = (kv ? value_slot<CH>(row, pc(i)) : key_piece<CH>(row, pc(i))) * 8;
           const char* p = (kv ? vc : kc) + offs[t & 3][kv][row] + c * 2;
           to_lds(FULL || c < a.D ? (const void*)p : att_zero, to + i * BLOCK * 16);
         }
       };
       if (rows)
-        walk((const T*)a.q + b * a.qs[0], a.qs[1], a.qs[2], [&](int i, const T* p, bool in) {
-          const int c = ((lane % CH) ^ kswz(lane / CH + 64 / CH * i)) * 8;
+        walk((const T*)a.q + b * a.qs[0], a.qs[1], a.qs[2], [&](int i, int row, int at, const T* p, bool in) {
+          const int c = key_piece<CH>(row, at) * 8;
           to_lds(in && (FULL || c < a.D) ? (const void*)(p + c) : att_zero, lds_at + own + i * 1024);
         });
       const int n_cached = cached - tile;  // (of this part; at most 0 when it has the nodes alone)
       if (n_cached > 0) {
         find(first + wave);
-        if (wave < 3) {
-          locate(wave);
-          find(first + wave + 4);
+        for (int k = wave; k < 3; k += TURN) {
+          locate(k);
+          find(first + k + TURN);
         }
       }
       wait_loads();
@@ -761,9 +794,9 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
       auto arrive = [&](int t, int buf) {
         wait_loads();     // this wave's pieces are in LDS
         __syncthreads();  // everyone's are; what the last tile was read from is free
-        if (wave == ((t + 3) & 3)) {
+        if (wave == ((t + 3) & (TURN - 1))) {
           locate(t + 3);
-          find(first + t + 7);
+          find(first + t + 3 + TURN);
         }
         if (t + 2 < n_cached) stage(t + 2, 0, buf);
         if (t + 1 < n_cached) stage(t + 1, 1, buf ^ 1);
@@ -772,12 +805,11 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
       // exponentials of another step's weights
       auto turn = [&](const f32x16* s, f32x16* n, int t, int buf) {
         const uint32_t vb = buf * TILE_BYTES, kb = vb ^ TILE_BYTES;
-        constexpr int KC = KSTEPS / 4;
         const float off = fmaf(-at_least(top), scale, Half<T>::bias);
         float part[2] = {0.f, 0.f};
         u32x4 p[4];
         auto keys = [&](int i) {
-          for (int k = i * KC; k < (i + 1) * KC; k++)
+          for (int k = i * KSTEPS / 4; k < (i + 1) * KSTEPS / 4; k++)
             for (int c = 0; c < 2; c++) {
               const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
               n[c] = mfma32(lds_read<u32x4>(koff[k], kb + c * 32 * CH * 16), qf[k], k ? n[c] : zero, T());
@@ -887,15 +919,15 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
         product(p, vb * TILE_BYTES);
       }
       if (!odd) continue;
-      // the sums of what went in as 0 (the finite values of its pieces with their weights), some of the channels at a time,
-      // in the LDS that the tile does not use
-      constexpr int TURNS = W / 2, DT = DP / TURNS;
-#pragma unroll
-      for (int turn = 0; turn < TURNS && rows; turn++) {
-        const int slice = wave * 32 + l32, d0 = turn * DT;
-        float* mine = (float*)(lds + (slice < ROWS / 2 ? (kb ^ 1) * TILE_BYTES : VBUF + (vb ^ 1) * TILE_BYTES)) + slice % (ROWS / 2) * DT;
+      // the sums of what went in as 0 (the finite values of its pieces with their weights), two waves at a time, in the LDS
+      // that the tile does not use
 #pragma unroll 1
-        for (int d = 4 * hh; d < DT; d += 8) *(f32x4*)(mine + d) = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int turn = 0; turn < W; turn += 2) {
+        if (turn) __syncthreads();
+        if (!rows || uni(wave) / 2 * 2 != turn) continue;
+        float* mine = (float*)(lds + (wave & 1 ? VBUF + (vb ^ 1) * TILE_BYTES : (kb ^ 1) * TILE_BYTES)) + l32 * DP;
+#pragma unroll 1
+        for (int d = 4 * hh; d < DP; d += 8) *(f32x4*)(mine + d) = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int j = 0; j < WIDE_TILE && base + j < a.N; j++) {
           if (m >= M || !(tr.anc[node][(base + j) / 32] >> (j % 32) & 1)) continue;
@@ -907,24 +939,23 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
           for (int e = 0; e < a.D; e++) dot = fmaf((float)q[e], (float)k[e], dot);
           const float w = __builtin_amdgcn_exp2f(fmaf((a.scale < 0.f ? -dot : dot) - at_least(top), scale, Half<T>::bias));
 #pragma unroll 1
-          for (int d = 4 * hh; d < DT && d0 + d < a.D; d += 8) {
-            if (!not_finite<T>(*(const u32x4*)(v + (d0 + d) / 8 * 8))) continue;
+          for (int d = 4 * hh; d < a.D; d += 8) {
+            if (!not_finite<T>(*(const u32x4*)(v + d / 8 * 8))) continue;
             for (int i = 0; i < 4; i++) {
-              const float y = (float)v[d0 + d + i];
+              const float y = (float)v[d + i];
               mine[d + i] += isfinite(y) ? w * y : y;
             }
           }
         }
         wave_order();
 #pragma unroll
-        for (int d = 0; d < DT / 32; d++)
+        for (int d = 0; d < DB; d++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             const f32x4 x = *(const f32x4*)(mine + 32 * d + 8 * i + 4 * hh);
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[turn * (DT / 32) + d][4 * i + e] += x[e];
+            for (int e = 0; e < 4; e++) o[d][4 * i + e] += x[e];
           }
-        wave_order();
       }
       __syncthreads();
       if (more) stage_nodes(tile);
@@ -949,16 +980,15 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void k_attend_wide(Attend
           if (sh.parts > 1)  // (an absent row's parts: a sum of 0)
             *(f32x4*)(a.part + at * a.D + x) = here ? y : none;
           else
-            *(uint64_t*)(lds + own + (l32 * CH + ((4 * d + i) ^ kswz(l32))) * 16 + 8 * hh) = here ? pack4<T>(y * f) : 0;
+            *(uint64_t*)(lds + own + (l32 * CH + key_slot<CH>(l32, 4 * d + i)) * 16 + 8 * hh) = here ? pack4<T>(y * f) : 0;
         }
     }
     if (sh.parts == 1 && rows) {
       wave_order();
       const int64_t line = (int64_t)a.Hq * a.D;
-      walk((const T*)a.out + (int64_t)b * a.N * line, line, a.D, [&](int i, const T* p, bool in) {
-        const int c = lane % CH, row = lane / CH + 64 / CH * i;
+      walk((const T*)a.out + (int64_t)b * a.N * line, line, a.D, [&](int, int row, int c, const T* p, bool in) {
         if (in && (FULL || c * 8 < a.D))
-          *(u32x4*)(const_cast<T*>(p) + c * 8) = *(const u32x4*)(lds + own + (row * CH + (c ^ kswz(row))) * 16);
+          *(u32x4*)(const_cast<T*>(p) + c * 8) = *(const u32x4*)(lds + own + (row * CH + key_slot<CH>(row, c)) * 16);
       });
     }
   }

@@ -497,6 +497,9 @@ ATTEND = [
     (1, 37, [257], 32, 2, 128, 128, "chain"),
     (2, 128, [40, 700], 2, 1, 256, 32, "random"),
     (1, 50, [65], 8, 1, 8, 1, "flat"),
+    # many tiles: 256 rows of 104, 64 rows of heads up to 32
+    (20, 70, [(i * 211) % 1100 + 300 for i in range(20)], 20, 5, 104, 64, "random"),
+    (26, 40, [(i * 211) % 1100 + 300 for i in range(26)], 7, 7, 24, 64, "random"),
     # 8 waves over few rows, and heads past 128 with one and more row tiles
     (33, 2, [(i * 71) % 1200 for i in range(33)], 8, 4, 104, 16, "chain"),
     (2, 16, [511, 513], 1, 1, 248, 64, "random"),
@@ -643,7 +646,7 @@ def test_attention_no_sequences():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N,Hq,D", [(30, 12, 128), (70, 4, 136), (12, 3, 256), (2, 4, 96)])
+@pytest.mark.parametrize("N,Hq,D", [(30, 12, 128), (70, 4, 136), (12, 3, 256), (2, 4, 96), (70, 4, 96), (40, 2, 32), (33, 1, 32)])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_attention_values_not_finite_by_shape(N, Hq, D, value):
     """The same where a workgroup has 256 rows, where heads are cut, and where there are few rows."""
@@ -652,6 +655,16 @@ def test_attention_values_not_finite_by_shape(N, Hq, D, value):
     c["v"][1, 0, 0, 0] = value            # the root: every row
     c["v"][2, N - 1, 0, :] = value
     check_attention(attend(on(c)), ref_attention(**c), BF)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N,Hq,Hkv,D", [(20, 70, 20, 5, 104), (26, 40, 7, 7, 24)])
+def test_attention_values_not_finite_among_many_tiles(B, N, Hq, Hkv, D):
+    c = make_attention(18, B, N, [(i * 211) % 1100 + 300 for i in range(B)], Hq, Hkv, D, 64, FP)
+    c["v"][0, N // 2, Hkv - 1, D - 1] = float("nan")
+    c["v"][1, 0, 0, 0] = -float("inf")
+    c["v"][B - 1, N - 1, :, :] = float("inf")
+    check_attention(attend(on(c)), ref_attention(**c), FP)
 
 
 @pytest.mark.gpu
