@@ -77,7 +77,12 @@ AttendPlan attend_plan(const geobpe_attend_args& x) {
   // eight waves where that fills the card without cutting the sequences (64 sequences x 4 heads: 26 us instead of 25 + 10
   // for the join); four where they are cut anyway, and more finely then (7 x 12 heads: 27 us instead of 40)
   p.waves = p.wide ? p.rows / 32 : x.head_dim <= 128 && items * p.row_tiles >= 128 && items * p.row_tiles <= 256 ? 8 : 4;
-  const int64_t want = ATT_WANT * 4 / p.waves, even = (items * p.row_tiles * tiles + want - 1) / want;
+  const int64_t want = ATT_WANT * 4 / p.waves;
+  int64_t even = (items * p.row_tiles * tiles + want - 1) / want;
+  // where whole parts are more than that after all, and a second round of workgroups would be a small one, they are half
+  // as long (86 x 4 heads over 4k to 8k positions, 688 workgroups: 193 us instead of 241; 12 x 2 over 33k to 66k, 528: 125
+  // instead of 160.  With 512 in the first place it takes longer: 16 x 2 heads over up to 12k 53 instead of 42)
+  if (even < tiles && items * p.row_tiles * ((tiles + even - 1) / even) > want) even = (even + 1) / 2;
   const int least = p.wide ? WIDE_LEAST : ATT_LEAST;
   p.per = (int)(even > tiles ? tiles : even > least ? even : least);
   p.most = (int)((tiles + p.per - 1) / p.per);

@@ -225,7 +225,7 @@ __device__ inline float* part_sums(const AttendArgs& a, int RT, int rows) {
 // LDS: K to be read in the operand's order, V for the transposing read; the rows there are 32 bytes longer than the head
 // so that eight of them start in different banks.
 template <typename T, int KS, int RB, int W>
-__global__ __launch_bounds__(64 * W, W > 4 || KS <= 2 || KS <= 4 && RB == 1 ? 2 : 1) void k_attend(AttendArgs a) {
+__global__ __launch_bounds__(64 * W, KS <= 4 ? 2 : 1) void k_attend(AttendArgs a) {
   constexpr int DP = 32 * KS, DB = 2 * KS, LROW = DP * 2 + 32;
   constexpr int DMIN = KS <= 4 ? DP - 24 : DP - 56;  // the heads this is for: DMIN .. DP
   constexpr int AREA = ATT_TILE * LROW;  // >= 16 rows of DP + 4 floats
@@ -874,7 +874,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_atte
         }
         arrive(t, t & 1);
         if (cached < last) {
-          nvb = t & 1 ^ 1;
+          nvb = (t & 1) ^ 1;
           stage_nodes(cached);
         }
         if (rows) {
