@@ -224,6 +224,11 @@ __device__ inline float* part_sums(const AttendArgs& a, int RT, int rows) {
 // product's operand wants, so nothing is moved between lanes but the maximum.  K and then V go through the wave's own
 // LDS: K to be read in the operand's order, V for the transposing read; the rows there are 32 bytes longer than the head
 // so that eight of them start in different banks.
+//
+// What bounds it is memory, or in small calls the way from one load to the next (lengths, table, keys, the join of the
+// waves: 6 us without a prefix).  64 chains of 5 nodes, 16 / 4 heads of 64, over 157 to 2237 positions: 24 us, 80 MB at
+// 3.3 TB/s, the longest chain's nine turns of its waves after another; one round of workgroups, so nothing evens that out
+// (cut finer 28 to 37 with the join).
 template <typename T, int KS, int RB, int W>
 __global__ __launch_bounds__(64 * W, KS <= 4 ? 2 : 1) void k_attend(AttendArgs a) {
   constexpr int DP = 32 * KS, DB = 2 * KS, LROW = DP * 2 + 32;
@@ -513,6 +518,12 @@ __global__ __launch_bounds__(64 * W, KS <= 4 ? 2 : 1) void k_attend(AttendArgs a
 // tiles of 64 keys from LDS.  Rows go there directly, the next tile's while this one's products run.
 // S^T = K Q^T and O^T = V^T P^T in the 32x32x16 instruction, in the same way as above: row = lane % 32, and a
 // lane's weights of four keys in a row are the second product's operand.
+//
+// Up to about 100 rows the cache's bytes bound it: 64 rows of heads of 128 over 131071 positions take 111 us and the
+// join 7, 537 MB at 4.8 TB/s.  Above it is the matrix units: 256 rows, 32 sequences over 8k to 16k: 500 to 550 us, 414
+// GFLOP at 750 to 830 TFLOP/s, where the card lowers its clock (the first launches take 480; no order of the
+// instructions, depth of the loads or priority of the waves made the later ones faster).  Small calls are the way from one
+// load to the next again: 432 rows without a prefix 9.6 us.
 //
 // In LDS a row's 16-byte pieces are permuted so that the operands' reads spread over the banks: eight rows' piece of K in
 // different ones (piece c of row r lies at c ^ (r & 7), in rows of 64 bytes at c ^ (r / 4 & 1), in those of 192, whose
@@ -995,7 +1006,8 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_atte
 }
 
 // Joins the parts: D / 4 threads a row, BY of them over its parts, J parts in flight each.  Rows of sequences with
-// one part were written already.
+// one part were written already.  4 us for few parts, of which 3 are the launch and its first loads; 512 rows of 128 of 63
+// parts 7.4 us (18 MB).
 template <typename T, int BY, int J>
 __global__ __launch_bounds__(ATT_BLOCK) void k_attend_join(AttendArgs a, int rows, int tile) {
   __shared__ f32x4 acc_[BY > 1 ? ATT_BLOCK : 1];

@@ -14,7 +14,9 @@
 // What has to be read: an entry of p and q for every node, and the rows of the contexts that a sum is needed of: the
 // last one's for the next id, others' only between a rejected child and its next sibling.  r is worked out anew from the
 // rows and the Z so far whenever it is needed, never stored.  One workgroup does a sequence: a row of 128 k entries takes
-// it about as long as the rows' share of the card's bandwidth once there are 100 sequences.
+// it about as long as the rows' share of the card's bandwidth once there are 100 sequences: 128 chains of 7 drafts over
+// 131072 fp32 entries take 34 us, 134 MB at 4.0 TB/s.  Small calls are dependent loads: one chain over 1091 ids 5.8 us, 48
+// trees of 40 nodes over 5123 ids 13.4 (the sequence with most rejected siblings, a sum each).
 #pragma once
 
 #include "draft.h"
