@@ -354,8 +354,10 @@ int geobpe_run_exchange_log(geobpe_ctx *ctx, int64_t n_merges, int64_t *n_done, 
  * sequence is absent), node i > 0 hangs on the present node parents[i] < i, else it is absent.
  * At most 128 nodes.  Device pointers on `device`, ordered on `stream` (a hipStream_t; NULL: the
  * default stream); nothing is allocated or waited for.  Strides are in elements (commit: bytes)
- * and may be any multiple of 16 bytes where rows of a head are meant.  GEOBPE_EARG: sizes,
- * alignment or a null pointer; the message is in geobpe_draft_error() (of this thread). */
+ * and may be any multiple of 16 bytes where rows of a head are meant (the attention's page and
+ * slot strides from 0 to below 64 GiB).  A table's positions, max_pages page_size, are at most
+ * 2^31 - 4096.  GEOBPE_EARG: sizes, alignment or a null pointer; the message is in
+ * geobpe_draft_error() (of this thread). */
 typedef struct {
   const void *d_q, *d_k_cache, *d_v_cache, *d_k, *d_v; /* queries; pages; the nodes' own keys and values */
   void *d_out;                                         /* seqs x nodes x heads x head_dim, contiguous */
@@ -398,7 +400,8 @@ typedef struct {
   int64_t layers, seqs, nodes, kv_heads, head_bytes, page_size, pages, max_pages;
 } geobpe_commit_args;
 /* cache[layer, position lens[b] + t] = node path[b, t] of sequence b for t < n[b]; lens_out = lens + n.
- * A kept node outside the tree, the table or the pages is not written, and lens_out[b] is -1. */
+ * A kept node outside the tree, the table or the pages is not written, and lens_out[b] is -1.  The
+ * nodes' rows, the caches and both lengths are memory of their own. */
 int geobpe_commit_draft(int device, void *stream, const geobpe_commit_args *args);
 const char *geobpe_draft_error(void);
 

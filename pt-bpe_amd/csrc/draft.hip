@@ -282,6 +282,7 @@ int geobpe_commit_draft(int device, void* stream, const geobpe_commit_args* p) {
   if (!x.d_k || !x.d_v || !x.d_k_cache || !x.d_v_cache || !x.d_lens || !x.d_path || !x.d_n || !x.d_lens_out ||
       (x.max_pages && !x.d_table))
     return fail(GEOBPE_EARG, "commit: null pointer");
+  if (x.d_lens_out == x.d_lens) return fail(GEOBPE_EARG, "commit: the new lengths would replace those that are still read");
   if (!aligned(x.d_k, x.k_stride, 4, 16) || !aligned(x.d_v, x.v_stride, 4, 16) ||
       !aligned(x.d_k_cache, x.kc_stride, 4, 16) || !aligned(x.d_v_cache, x.vc_stride, 4, 16))
     return fail(GEOBPE_EARG, "commit: rows are not 16-byte aligned");

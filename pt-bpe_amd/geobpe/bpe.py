@@ -510,9 +510,10 @@ class BPE:
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         kept = self.__dict__.setdefault("_id_ranges", {})
-        if (K, device) not in kept:
-            kept[K, device] = torch.tensor(r, device=device)
-        return kept[K, device]
+        key = (r.tobytes(), device)
+        if key not in kept:
+            kept[key] = torch.tensor(r, device=device)
+        return kept[key]
 
     def verify_draft(self, parents, ids, target, draft, u, start):
         """Drafted ids against a model's probabilities over this vocabulary (geobpe.draft.verify), each place

@@ -64,7 +64,8 @@ def tree_attention(q, k_cache, v_cache, block_table, lens, k, v, parents, scale:
     multiple of 8 up to 256, Hq a multiple of Hkv (query head h reads kv head h // (Hq // Hkv)).
     k_cache, v_cache (pages, page size, Hkv, D): position x of sequence b is slot x % page size of page
     block_table[b, x // page size]; lens (B,): its committed positions.  Other orders of the cache's
-    dimensions are views with strides (16-byte aligned rows).  scale: D ** -0.5 if None.
+    dimensions are views with strides (16-byte aligned rows).  scale: D ** -0.5 if None.  A call has at most
+    2^23 - 1 query rows (B N Hq) and a table MAX_POSITIONS positions.
 
     Returns (B, N, Hq, D).  Rows of absent nodes are 0 whatever their keys and values hold, and so does
     nothing outside a node's own path reach its row.  A length outside the table, or a page outside the cache
@@ -86,7 +87,7 @@ def verify(parents, ids, target, draft, u, ranges=None, start=None) -> Verified:
     ids (B, N) int32 or int64 (ids[:, 0] is not read; an id outside the vocabulary is rejected), target and draft
     (B, N, V) of one type (float32, bfloat16, float16; the rows are used as they are, entries that are not finite and
     positive count as 0), row i the distribution after node i; draft None: drafts without probabilities, draft(x)
-    is 1 at the drafted id.  u (B, N) float32.
+    is 1 at the drafted id.  u (B, N) float32 (NaN keeps no child; beyond [0, 1) the next id is the first or last one with mass).
     ranges (C, 2) int32 and start (B,) int32: the token after node i is at place start[b] + depth(i), and outside
     ranges[place % C] = [lo, hi) a row's entries are taken as 0 and not read (``BPE.id_ranges``)."""
     return Verified(*(_bound or _ops()).verify(parents, ids, target, draft, u, ranges, start))
@@ -99,7 +100,8 @@ def commit(k_cache, v_cache, block_table, lens, k, v, path, n):
     k_cache, v_cache (pages, page size, Hkv, D) and k, v (B, N, Hkv, D), or with a leading dimension of layers, of
     any type whose rows are multiples of 16 bytes; path (B, N) and n (B,) as ``verify`` returns them.  The table has
     to have the pages for the new positions.  A kept node outside the tree, the table or the cache is not written,
-    and that sequence's new length is -1.  Pages that sequences share must not be among the written ones."""
+    and that sequence's new length is -1.  Pages that sequences share must not be among the written ones, k and v not lie
+    in the cache's own memory, and a cache for both keys and values is refused."""
     return (_bound or _ops()).commit(k_cache, v_cache, block_table, lens, k, v, path, n)
 
 

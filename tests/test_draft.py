@@ -379,6 +379,8 @@ def test_c_entries_refuse_without_a_device():
         sizes = [bad if j == i else x for j, x in enumerate([1, 2, 4, 2, 128, 16, 3, 2])]
         assert L.geobpe_commit_draft(0, None, _COMMIT.pack(*k, *sizes)) == _native.E_ARG, (i, bad)
     assert L.geobpe_commit_draft(0, None, _COMMIT.pack(*k[:9], 8, *k[10:], 1, 2, 4, 2, 128, 16, 3, 2)) == _native.E_ARG
+    assert L.geobpe_commit_draft(0, None, _COMMIT.pack(*k, 1, 2, 4, 2, 128, 16, 3, 2)) == _native.E_ARG
+    assert b"new lengths" in L.geobpe_draft_error()  # (they are the old ones' memory here)
 
 
 @pytest.fixture(scope="module")

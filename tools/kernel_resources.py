@@ -1,4 +1,4 @@
-"""VGPRs, AGPRs, scratch (register spills) and occupancy of every kernel of csrc/geobpe.hip for
+"""VGPRs, AGPRs, scratch (register spills) and occupancy of every kernel of csrc/geobpe.hip and csrc/draft.hip for
 gfx950, from the compiler's resource-usage remarks (device-only compile, nothing written).
 
   python tools/kernel_resources.py [filter] [-- extra hipcc flags]"""
@@ -12,8 +12,9 @@ argv = sys.argv[1:]
 extra = argv[argv.index("--") + 1:] if "--" in argv else []
 flt = argv[0] if argv and argv[0] != "--" else ""
 cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "--cuda-device-only", "-c", "-o",
-       "/dev/null", "-Rpass-analysis=kernel-resource-usage", *extra, os.path.join(ROOT, "pt-bpe_amd/csrc/geobpe.hip")]
-out = subprocess.run(cmd, capture_output=True, text=True).stderr
+       "/dev/null", "-Rpass-analysis=kernel-resource-usage", *extra]
+out = "".join(subprocess.run([*cmd, os.path.join(ROOT, "pt-bpe_amd/csrc", f)], capture_output=True, text=True).stderr
+              for f in ("geobpe.hip", "draft.hip"))
 rows, cur = {}, None
 for ln in out.splitlines():
     m = re.search(r"Function Name: (\S+)", ln)
