@@ -69,25 +69,30 @@ AttendPlan attend_plan(const geobpe_attend_args& x) {
   // 114).  Where they are few 128 make more workgroups (2 heads of 432 rows over 960: 18 us instead of 22; 16 heads of 40
   // rows over 3k: 14.1 instead of 16.0).
   const bool many = items * ((M + 255) / 256) * tiles >= WIDE_MANY;
-  p.rows = !p.wide                                                            ? 16 * p.rb
+  p.rows = !p.wide ? 16 * p.rb
            : many && M > 128 && x.head_dim > 96 && x.head_dim <= 128 ? 256
-           : many && M <= 64 && x.head_dim <= 32                     ? 64
-                                                                     : 128;
+           : many && M <= 64 && x.head_dim <= 32 ? 64 : 128;
   p.row_tiles = (M + p.rows - 1) / p.rows;
-  // eight waves where that fills the card without cutting the sequences (64 sequences x 4 heads: 26 us instead of 25 + 10
-  // for the join); four where they are cut anyway, and more finely then (7 x 12 heads: 27 us instead of 40)
-  p.waves = p.wide ? p.rows / 32 : x.head_dim <= 128 && items * p.row_tiles >= 128 && items * p.row_tiles <= 256 ? 8 : 4;
+  // With few rows eight waves where sequences need not be cut then: 128 to 256 workgroups (64 sequences x 4 heads: 26 us
+  // instead of 25 + 10 for the join; 160 x 1000 positions 16 instead of 24), or 17 to 32 tiles (600 positions 10.0 instead of
+  // 12.0; at 33 tiles of heads of 128 17.4 instead of 16.1); else four, and finer parts (7 x 12 heads: 27 us instead of 40).
+  const int64_t uncut = items * p.row_tiles;
+  const bool eight = x.head_dim <= 128 && uncut <= 256 && (uncut >= 128 || (tiles > ATT_LEAST && tiles <= 32));
+  p.waves = p.wide ? p.rows / 32 : eight ? 8 : 4;
   const int64_t want = ATT_WANT * 4 / p.waves;
-  int64_t even = (items * p.row_tiles * tiles + want - 1) / want;
+  int64_t even = (uncut * tiles + want - 1) / want;
   // where whole parts are more than that after all, and a second round of workgroups would be a small one, they are half
   // as long (86 x 4 heads over 4k to 8k positions, 688 workgroups: 193 us instead of 241; 12 x 2 over 33k to 66k, 528: 125
   // instead of 160.  With 512 in the first place it takes longer: 16 x 2 heads over up to 12k 53 instead of 42)
-  if (even < tiles && items * p.row_tiles * ((tiles + even - 1) / even) > want) even = (even + 1) / 2;
-  const int least = p.wide ? WIDE_LEAST : ATT_LEAST;
+  if (even < tiles && uncut * ((tiles + even - 1) / even) > want) even = (even + 1) / 2;
+  // the least tiles of a part; uncut ones with eight waves are longer (160 sequences of 2000 or 8000 positions: 23 us instead
+  // of 34, 64 instead of 72), and so are those of more than 256 workgroups (320 over up to 3000 positions 84 us instead of
+  // 103; but 400 over up to 4000 74 instead of 66)
+  const int least = p.wide ? WIDE_LEAST : p.waves == 8 ? 256 : uncut > 256 && tiles <= 96 ? 96 : ATT_LEAST;
   p.per = (int)(even > tiles ? tiles : even > least ? even : least);
   p.most = (int)((tiles + p.per - 1) / p.per);
   p.blocks = (items * p.most + 7) / 8 * 8 * p.row_tiles;
-  p.bytes = p.most > 1 ? items * p.row_tiles * p.most * p.rows * (x.head_dim + 2) * 4 : 0;
+  p.bytes = p.most > 1 ? uncut * p.most * p.rows * (x.head_dim + 2) * 4 : 0;
   return p;
 }
 int attend_sizes(const geobpe_attend_args& x) {

@@ -378,7 +378,8 @@ def test_c_entries_refuse_without_a_device():
     for i, bad in ((0, 0), (1, -1), (2, 0), (3, 0), (4, 24), (5, 0), (6, 0), (7, -1)):
         sizes = [bad if j == i else x for j, x in enumerate([1, 2, 4, 2, 128, 16, 3, 2])]
         assert L.geobpe_commit_draft(0, None, _COMMIT.pack(*k, *sizes)) == _native.E_ARG, (i, bad)
-    assert L.geobpe_commit_draft(0, None, _COMMIT.pack(*k[:9], 8, *k[10:], 1, 2, 4, 2, 128, 16, 3, 2)) == _native.E_ARG
+    assert L.geobpe_commit_draft(0, None, _COMMIT.pack(*k[:8], 512, 8, *k[10:], 1, 2, 4, 2, 128, 16, 3, 2)) == _native.E_ARG
+    assert b"aligned" in L.geobpe_draft_error()
     assert L.geobpe_commit_draft(0, None, _COMMIT.pack(*k, 1, 2, 4, 2, 128, 16, 3, 2)) == _native.E_ARG
     assert b"new lengths" in L.geobpe_draft_error()  # (they are the old ones' memory here)
 
@@ -499,6 +500,10 @@ ATTEND = [
     (1, 37, [257], 32, 2, 128, 128, "chain"),
     (2, 128, [40, 700], 2, 1, 256, 32, "random"),
     (1, 50, [65], 8, 1, 8, 1, "flat"),
+    # eight waves over one part: 17 to 32 tiles
+    (1, 3, [700], 4, 4, 64, 16, "chain"),
+    (2, 7, [601, 540], 8, 2, 128, 16, "random"),
+    (3, 2, [960, 0, 33], 4, 2, 40, 24, "chain"),
     # many tiles: 256 rows of 104, 64 rows of heads up to 32
     (20, 70, [(i * 211) % 1100 + 300 for i in range(20)], 20, 5, 104, 64, "random"),
     (26, 40, [(i * 211) % 1100 + 300 for i in range(26)], 7, 7, 24, 64, "random"),
