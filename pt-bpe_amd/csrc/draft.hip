@@ -85,10 +85,11 @@ AttendPlan attend_plan(const geobpe_attend_args& x) {
   // as long (86 x 4 heads over 4k to 8k positions, 688 workgroups: 193 us instead of 241; 12 x 2 over 33k to 66k, 528: 125
   // instead of 160.  With 512 in the first place it takes longer: 16 x 2 heads over up to 12k 53 instead of 42)
   if (even < tiles && uncut * ((tiles + even - 1) / even) > want) even = (even + 1) / 2;
-  // the least tiles of a part; uncut ones with eight waves are longer (160 sequences of 2000 or 8000 positions: 23 us instead
-  // of 34, 64 instead of 72), and so are those of more than 256 workgroups (320 over up to 3000 positions 84 us instead of
-  // 103; but 400 over up to 4000 74 instead of 66)
-  const int least = p.wide ? WIDE_LEAST : p.waves == 8 ? 256 : uncut > 256 && tiles <= 96 ? 96 : ATT_LEAST;
+  // The least tiles of a part.  Sequences stay whole up to 256 tiles with eight waves and few rows (160 sequences of 2000 or
+  // 8000 positions: 23 us instead of 34, 64 instead of 72), and up to 96 where they make a round of workgroups without a
+  // cut: few rows, 320 over up to 3000 positions 84 us instead of 103 (but 400 over up to 4000 74 instead of 66); many,
+  // 480 over 2000 64 instead of 83, 320 over 3k to 6k 201 instead of 227 (but 344 over 4k to 8k 219 instead of 194).
+  const int least = !p.wide && p.waves == 8 ? 256 : uncut >= 256 && tiles <= 96 ? 96 : p.wide ? WIDE_LEAST : ATT_LEAST;
   p.per = (int)(even > tiles ? tiles : even > least ? even : least);
   p.most = (int)((tiles + p.per - 1) / p.per);
   p.blocks = (items * p.most + 7) / 8 * 8 * p.row_tiles;
