@@ -96,15 +96,14 @@ AttendPlan attend_plan(const geobpe_attend_args& x) {
   p.bytes = p.most > 1 ? uncut * p.most * p.rows * (x.head_dim + 2) * 4 : 0;
   return p;
 }
-int attend_sizes(const geobpe_attend_args& x) {
+int attend_sizes(const geobpe_attend_args& x, AttendPlan& plan) {
   if (x.seqs < 0 || x.nodes < 1 || x.nodes > DRAFT_MAX_NODES || x.kv_heads < 1 || x.heads < x.kv_heads ||
       x.heads % x.kv_heads || x.head_dim < 8 || x.head_dim > 256 || x.head_dim % 8 || x.page_size < 1 || x.pages < 1 ||
       x.max_pages < 0 || x.dtype < 0 || x.dtype > 1 || x.seqs > 65535 || x.heads > 65535 || x.pages > INT32_MAX ||
       x.page_size > DRAFT_MAX_POSITIONS || x.max_pages > DRAFT_MAX_POSITIONS / x.page_size)
     return fail(GEOBPE_EARG, "tree attention: sizes out of range");
   if (x.seqs == 0) return GEOBPE_OK;
-  if (x.seqs * x.nodes * x.heads > INT32_MAX / ATT_BLOCK ||
-      attend_plan(x).blocks > INT32_MAX / ATT_BLOCK)
+  if (x.seqs * x.nodes * x.heads > INT32_MAX / ATT_BLOCK || (plan = attend_plan(x)).blocks > INT32_MAX / ATT_BLOCK)
     return fail(GEOBPE_EARG, "tree attention: %lld sequences of %lld rows are too many for one call", (long long)x.seqs,
                 (long long)(x.nodes * x.heads));
   return GEOBPE_OK;
@@ -197,16 +196,17 @@ extern "C" {
 const char* geobpe_draft_error(void) { return g_draft_error; }
 
 int64_t geobpe_tree_attention_work(const geobpe_attend_args* p) {
-  if (!p || attend_sizes(*p) != GEOBPE_OK) return -1;
-  return p->seqs ? attend_plan(*p).bytes : 0;
+  AttendPlan plan;
+  if (!p || attend_sizes(*p, plan) != GEOBPE_OK) return -1;
+  return p->seqs ? plan.bytes : 0;
 }
 
 int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p, void* d_work, int64_t work_bytes) {
   if (!p) return fail(GEOBPE_EARG, "no arguments");
   const geobpe_attend_args& x = *p;
-  const int rc = attend_sizes(x);
+  AttendPlan plan;
+  const int rc = attend_sizes(x, plan);
   if (rc != GEOBPE_OK || x.seqs == 0) return rc;
-  const AttendPlan plan = attend_plan(x);
   if (!x.d_q || !x.d_k_cache || !x.d_v_cache || !x.d_k || !x.d_v || !x.d_lens || !x.d_parents || !x.d_out ||
       (x.max_pages && !x.d_table) || (plan.bytes && !d_work))
     return fail(GEOBPE_EARG, "tree attention: null pointer");

@@ -884,6 +884,27 @@ def test_verify_numbers_outside(drafted):
 
 
 @pytest.mark.gpu
+def test_verify_outputs_are_tensors_of_their_own():
+    """The three results share an allocation and nothing else: contiguous, written to alone, in inference mode too, kept
+    after the others are gone; none for no sequences."""
+    c = make_verify(19, 5, 7, 40, torch.float32, "random")
+    d, want = on(c), ref_verify(c["parents"], c["ids"], c["target"], c["draft"], c["u"])
+    for inference in (False, True):
+        with torch.inference_mode(inference):
+            got = verify(d)
+            assert [x.shape for x in got] == [(5,), (5, 7), (5, 7)] and all(x.is_contiguous() and x.dtype == torch.int32 for x in got)
+            assert got.n.is_inference() == inference and not got.path.requires_grad
+            got.path.fill_(-9)
+            assert np.array_equal(got.n.cpu(), want[0]) and np.array_equal(got.tokens.cpu(), want[2])
+            tokens = got.tokens
+            del got
+            torch.empty(5 * 15, dtype=torch.int32, device="cuda").fill_(3)
+            assert np.array_equal(tokens.cpu(), want[2]) and torch.equal((tokens + 1).cpu(), torch.tensor(want[2] + 1, dtype=torch.int32))
+    e = {k: v[:0] for k, v in d.items() if isinstance(v, torch.Tensor)}
+    assert [x.shape for x in verify({**d, **e})] == [(0,), (0, 7), (0, 7)]
+
+
+@pytest.mark.gpu
 def test_verify_captured():
     """Replays over new numbers, with eager calls between; shared rows (stride 0)."""
     c = make_verify(17, 4, 8, 9000, torch.float32, "random")
