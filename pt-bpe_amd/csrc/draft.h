@@ -31,6 +31,18 @@ __device__ inline void draft_climb(DraftNode& n, const DraftNode& above) {
   for (int k = 0; k < DRAFT_MAX_NODES / 32; k++) n.w[k] |= above.w[k];
 }
 
+// Which of a tree's tiles of DRAFT_TILE nodes hold a value that is not finite, in LDS.  A flag each: a wave may be at the next
+// tile's before another has read this one's, and the barriers that follow hang on what is read.
+constexpr int DRAFT_TILE = 64;
+struct TileFlags {
+  int of[DRAFT_MAX_NODES / DRAFT_TILE];
+  __device__ void clear() {
+    for (int& f : of) f = 0;
+  }
+  __device__ void mark(int node) { of[node / DRAFT_TILE] = 1; }
+  __device__ bool marked(int node) const { return of[node / DRAFT_TILE] != 0; }
+};
+
 // x / d for 0 <= x < 2^31 and 1 <= d < 2^31, with the host's m = min(2^32 / d, 2^32 - 1) rounded down: x m / 2^32
 // is at most x / d and below it by less than x / 2^32 < 1/2, so its floor is the quotient or one less, which the
 // remainder tells.

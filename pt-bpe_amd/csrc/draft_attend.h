@@ -551,7 +551,7 @@ __device__ inline int value_slot(int row, int c) {  // (its own inverse)
 }
 // A part has at least 4 tiles (2 heads of 432 rows over 960 positions, at least 16 / 8 / 4 / 2 tiles: 36 / 22 / 18 / 15.5 us;
 // with 2 those over 64 took 13.2 instead of 11.0 for the join).  `Many` tiles: eight for every CU.
-constexpr int WIDE_TILE = 64, WIDE_LEAST = 4, WIDE_MANY = 2048;
+constexpr int WIDE_TILE = DRAFT_TILE, WIDE_LEAST = 4, WIDE_MANY = 2048;
 constexpr float SLACK = 8.f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -609,7 +609,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_atte
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];  // K of two tiles, V of two
   __shared__ uint64_t offs[4][2][WIDE_TILE];                         // the rows' places in the cache: tile % 4, K or V
   __shared__ Tree tr;
-  __shared__ int odd_;
+  __shared__ TileFlags odd_;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, hh = lane >> 5;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   const float scale = score_scale(a.scale);
@@ -736,7 +736,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_atte
 
     {
       const int len = uni(sp.len);
-      if (t == 0) odd_ = 0;
+      if (t == 0) odd_.clear();
       const Parents parents = tree_parents(a.N, a.parents + b * a.parents_stride);
       const Pages pages = {a.table + b * a.table_stride, a.div, a.P, a.M};
       const char* kc = (const char*)((const T*)a.kc + h * a.khead);
@@ -906,12 +906,12 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_atte
         u32x4* at = (u32x4*)(lds + VBUF + nvb * TILE_BYTES + (t + BLOCK * i) * 16);
         if (not_finite<T>(*at)) {
           *at = u32x4{0, 0, 0, 0};
-          odd_ = 1;
+          odd_.mark(base);
         }
       }
       __syncthreads();
       const int kb = nkb, vb = nvb;
-      const bool more = ++tile < last, odd = odd_;
+      const bool more = ++tile < last, odd = odd_.marked(base);
       if (more && !odd) {  // (else the other buffers are needed below)
         nkb ^= 1;
         nvb ^= 1;
