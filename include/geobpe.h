@@ -386,7 +386,9 @@ typedef struct {
 } geobpe_verify_args;
 /* Per sequence: node i's id is accepted when u[i] draft[parent, id] Z < r(id), r the target's row of
  * the parent less what its rejected siblings took (r <- max(r - Z draft, 0), Z <- sum r, at first 1);
- * the next id is the first whose cumulative r passes u[0] sum r.  n: the kept nodes, root
+ * the next id is the first whose cumulative r passes u[0] sum r.  With classes, the token after node i
+ * is at place start + depth(i): rows are read inside [lo, hi) = ranges[place % classes] only and divided by
+ * their mass there, and a drafted id outside is passed over.  n: the kept nodes, root
  * included; path: their indices; tokens: the n - 1 accepted ids, then the next one; -1 behind. */
 int geobpe_verify_draft(int device, void *stream, const geobpe_verify_args *args);
 

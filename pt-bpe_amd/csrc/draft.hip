@@ -175,19 +175,19 @@ void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
   }
 }
 
-template <typename T, int W>
+template <typename T, bool HELD, int W>
 void verify_waves(const VerifyArgs& a, hipStream_t s) {
   if (a.draft)
-    hipLaunchKernelGGL((k_verify<T, true, W>), dim3((unsigned)a.B), dim3(64 * W), 0, s, a);
+    hipLaunchKernelGGL((k_verify<T, true, HELD, W>), dim3((unsigned)a.B), dim3(64 * W), 0, s, a);
   else
-    hipLaunchKernelGGL((k_verify<T, false, W>), dim3((unsigned)a.B), dim3(64 * W), 0, s, a);
+    hipLaunchKernelGGL((k_verify<T, false, HELD, W>), dim3((unsigned)a.B), dim3(64 * W), 0, s, a);
 }
 template <typename T>
 void verify_launch(const VerifyArgs& a, hipStream_t s) {
   if (a.V <= VER_SMALL)
-    verify_waves<T, 4>(a, s);
+    a.C ? verify_waves<T, true, 4>(a, s) : verify_waves<T, false, 4>(a, s);
   else
-    verify_waves<T, 16>(a, s);
+    a.C ? verify_waves<T, true, 16>(a, s) : verify_waves<T, false, 16>(a, s);
 }
 }  // namespace
 

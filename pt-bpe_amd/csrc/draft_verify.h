@@ -6,17 +6,25 @@
 //     else:                  r <- max(r - Z q_c, 0), Z = sum r
 //   next id: the smallest x with sum_{y <= x} r(y) > u[0] sum r;  r without mass: from p_c
 //
+// With ranges a row counts as what it is inside the range of its place, divided by its mass there: p / P, q / Q.  Kept
+// times P, r still starts as the row's own entries; then Z = sum r / Q, P / Q at first (without draft rows sum r, P at first).
+// A drafted id outside the range says nothing of those inside: it is passed over, as is every one of a draft row without
+// mass there.  A P or Q that is 1 but for the type's rounding is taken as 1: rows that were normalised there are used as
+// they are, as all are without ranges (so ranges that leave nothing out change nothing).
+//
 // Children come after their parents, so one ascending pass visits every context's children.
 // Without draft rows q_c is one at the drafted id: r loses that entry.  Probabilities are read
 // as they are (finite positive entries, others 0); sums, products and comparisons are in 64 bits,
 // so an id near a border of two of them does not hang on the order of the sums.
 //
 // What has to be read: an entry of p and q for every node, and the rows of the contexts that a sum is needed of: the
-// last one's for the next id, others' only between a rejected child and its next sibling.  r is worked out anew from the
+// last one's for the next id, others' only between a rejected child and its next sibling, and with ranges once for P and Q
+// of those with drafted children.  r is worked out anew from the
 // rows and the Z so far whenever it is needed, never stored.  One workgroup does a sequence: a row of 128 k entries takes
 // it about as long as the rows' share of the card's bandwidth once there are 100 sequences: 128 chains of 7 drafts over
-// 131072 fp32 entries take 34 us, 134 MB at 4.0 TB/s.  Small calls are dependent loads: one chain over 1091 ids 5.8 us, 48
-// trees of 40 nodes over 5123 ids 13.4 (the sequence with most rejected siblings, a sum each).
+// 131072 fp32 entries take 34 us, 134 MB at 4.0 TB/s.  Small calls are dependent loads: one chain over 1091 ids 5.3 us, 48
+// trees of 40 nodes over 5123 ids held to ranges 18.5 (the longest walk: a sum for every context with children, and one per
+// rejected sibling).
 #pragma once
 
 #include "draft.h"
@@ -54,8 +62,16 @@ __device__ inline float prob(T v) {
   return __builtin_amdgcn_classf(f, 0x180) ? f : 0.f;  // positive, finite
 }
 
+// a mass as the rows are divided by it: a row normalised in 32 bits (2^-20 for its sums) and rounded once has 1 to within
+// half a step of T
+template <typename T>
+__device__ inline double mass_of(double m) {
+  constexpr double half = sizeof(T) == 4 ? 0x1p-24 : __is_same(T, _Float16) ? 0x1p-11 : 0x1p-8;
+  return fabs(m - 1.0) <= half + 0x1p-20 ? 1.0 : m;
+}
+
 // a context's row with what its rejected children took
-template <typename T, bool Q>
+template <typename T, bool Q, bool HELD>
 struct VerRow {
   static constexpr int VEC = 16 / sizeof(T);
   const T *p, *q;
@@ -98,11 +114,11 @@ struct VerRow {
 #pragma unroll
     for (int k = 0; k < VEC; k++) r[k] = pv[k];
     if (Q) {
-      if (rejected) {  // (Z of the first is 1)
+      if (!HELD && rejected) {  // (Z of the first is 1)
 #pragma unroll
         for (int k = 0; k < VEC; k++) r[k] = fmax(r[k] - (double)qv[k], 0.0);
       }
-      for (int j = 1; j < rejected; j++) {
+      for (int j = !HELD; j < rejected; j++) {
         const double z = Z[j];
 #pragma unroll
         for (int k = 0; k < VEC; k++) r[k] = fmax(fma(-z, (double)qv[k], r[k]), 0.0);
@@ -152,10 +168,11 @@ __device__ inline double wave_total(double v) { return lane_value(wave_scan(v), 
 __device__ inline float lane_value(float v, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l)); }
 
 // One workgroup of W waves per sequence.  Every wave holds the whole tree (nodes lane and lane + 64) and makes the same
-// walk; they part only over the rows.
-template <typename T, bool Q, int W>
+// walk; they part only over the rows.  HELD: with ranges (a kernel of its own, for its sums of P and Q make the others' code
+// longer: 5.9 us instead of 5.3 for one chain without ranges).
+template <typename T, bool Q, bool HELD, int W>
 __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
-  typedef VerRow<T, Q> Row;
+  typedef VerRow<T, Q, HELD> Row;
   constexpr int VEC = Row::VEC, STEP = 64 * VEC, DEEP = (Q && W > 4 ? 16 : 32) / VEC;  // steps in flight (with 16 waves 128 registers have to hold them)
   __shared__ double Z[DRAFT_MAX_NODES], part[W];
   __shared__ int rejx[DRAFT_MAX_NODES];
@@ -163,7 +180,7 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b = blockIdx.x, N = a.N;
   const T* target = (const T*)a.target + b * a.ts[0];
   const T* draft = (const T*)a.draft + b * a.ds[0];
-  const int start = a.C ? a.start[b] : 0;
+  const int start = HELD ? a.start[b] : 0;
 
   int par[2], id[2], up[2], depth[2];
   float u[2], P[2] = {0.f, 0.f}, q[2];
@@ -198,7 +215,7 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
   auto range = [&](int d, int& lo, int& hi) {
     lo = 0;
     hi = a.V;
-    if (!a.C) return;
+    if (!HELD) return;
     int c = (int)(((int64_t)start + d) % a.C);
     if (c < 0) c += a.C;
     lo = max(a.ranges[2 * c], 0);
@@ -250,18 +267,52 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
     return wave_total(all);
   };
 
+  // P, and Qs, the mass of the draft's row, as sums in one order: equal rows have equal ones.  Up to 64 entries every wave
+  // sums itself.
+  auto masses = [&](int lo, int hi, double& Qs) {
+    __shared__ double part_q[W];
+    double s = 0, sq = 0;
+    if (hi - lo <= 64) {
+      if (lo + lane < hi) s = prob(row.p[lo + lane]), sq = prob(row.q[lo + lane]);
+      Qs = wave_total(sq);
+      return wave_total(s);
+    }
+#pragma unroll 8
+    for (int i = lo + t; i < hi; i += 64 * W) s += prob(row.p[i]), sq += prob(row.q[i]);
+    s = wave_total(s), sq = wave_total(sq);
+    __syncthreads();
+    if (lane == 0) part[wave] = s, part_q[wave] = sq;
+    __syncthreads();
+    Qs = wave_total(lane < W ? part_q[lane] : 0.0);
+    return wave_total(lane < W ? part[lane] : 0.0);
+  };
+
   int c = 0, n = 1, seen = 0;
   double z = 1.0, full = 0;
+  row.rejected = 0;
   if (t == 0) path[0] = 0;
   for (;;) {
     row.p = target + c * a.ts[1];
     row.q = draft + c * a.ds[1];
     range(n - 1, row.lo, row.hi);
+    // Z of the first child differs from context to context with ranges: no wave may still read the last one's
+    if (Q && HELD && row.rejected) __syncthreads();
     row.rejected = 0;
     z = 1.0;    // Z (-1: to be taken)
     full = 0;   // without draft rows the last one that was taken,
     seen = 0;   // and the children rejected by then
     uint64_t kids[2] = {__ballot(here[0] && par[0] == c && lane > 0), __ballot(here[1] && par[1] == c)};
+    double Qs = 1.0;
+    if constexpr (HELD) {
+      for (int k = 0; k < 2; k++) kids[k] &= __ballot(id[k] >= row.lo && id[k] < row.hi);
+      z = -1.0;
+      if (Q && (kids[0] | kids[1])) {
+        z = mass_of<T>(masses(row.lo, row.hi, Qs));
+        Qs = mass_of<T>(Qs);
+        if (!(Qs > 0)) kids[0] = kids[1] = 0;
+        z /= Qs;
+      }
+    }
     int taken = -1;
     uint64_t gone[2] = {0, 0};
     while (kids[0] | kids[1]) {
@@ -270,11 +321,12 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
       const int x = __builtin_amdgcn_readlane(k ? id[1] : id[0], l);
       const double qx = lane_value(k ? q[1] : q[0], l), ux = lane_value(k ? u[1] : u[0], l);
       double r = lane_value(k ? P[1] : P[0], l);
+      if ((HELD || row.rejected) && z < 0) {
+        full = sums(row.lo, row.hi);
+        seen = row.rejected;
+        z = !HELD ? full : Q ? full / Qs : row.rejected ? full : mass_of<T>(full);
+      }
       if (row.rejected) {
-        if (z < 0) {
-          z = full = sums(row.lo, row.hi);
-          seen = row.rejected;
-        }
         if (Q) {
           for (int j = 0; j < row.rejected; j++) r = fmax(fma(-Z[j], qx, r), 0.0);
         } else {
@@ -289,7 +341,8 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
         }
         break;
       }
-      // (every wave writes the same, and no wave is in another context while one reads: both read in sums)
+      // (every wave writes the same.  The first entry of a context may be written while a slower wave still reads the last
+      // context's, which is the same 1, or is kept from it above; before the second there is a sum and its barriers)
       if (Q) {
         Z[row.rejected] = z;
         z = -1.0;
@@ -298,6 +351,7 @@ __global__ __launch_bounds__(64 * W) void k_verify(VerifyArgs a) {
         gone[k] |= 1ull << l;
         rejx[row.rejected] = x;
         rejr[row.rejected] = r;
+        if (HELD && !row.rejected) z = full;
         z = full > 0 && z - r > VER_KEEP * full ? z - r : -1.0;
       }
       row.rejected++;

@@ -518,8 +518,9 @@ class BPE:
     def verify_draft(self, parents, ids, target, draft, u, start):
         """Drafted ids against a model's probabilities over this vocabulary (geobpe.draft.verify), each place
         held to its kind of id (``id_ranges``): start[b] is the place in the chain of the token after the root,
-        i.e. the number of ids decided so far.  A row may be wider than vocab_size (a model's own extra ids lie
-        behind it); those are never drawn here.  ``tokens`` of the result is what dequantize / recover take."""
+        i.e. the number of ids decided so far.  Rows are the model's own, over all ids: a place's are divided by their
+        mass there.  A row may be wider than vocab_size (a model's own extra ids lie behind it); those are never
+        drawn here.  ``tokens`` of the result is what dequantize / recover take."""
         from . import draft as _draft
         if target.shape[-1] < self.vocab_size:
             raise ValueError(f"rows of {target.shape[-1]} probabilities for {self.vocab_size} ids")

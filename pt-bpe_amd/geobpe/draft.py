@@ -88,8 +88,11 @@ def verify(parents, ids, target, draft, u, ranges=None, start=None) -> Verified:
     (B, N, V) of one type (float32, bfloat16, float16; the rows are used as they are, entries that are not finite and
     positive count as 0), row i the distribution after node i; draft None: drafts without probabilities, draft(x)
     is 1 at the drafted id.  u (B, N) float32 (NaN keeps no child; beyond [0, 1) the next id is the first or last one with mass).
-    ranges (C, 2) int32 and start (B,) int32: the token after node i is at place start[b] + depth(i), and outside
-    ranges[place % C] = [lo, hi) a row's entries are taken as 0 and not read (``BPE.id_ranges``)."""
+    ranges (C, 2) int32 and start (B,) int32: the token after node i is at place start[b] + depth(i), and the rows after it
+    count as what they are inside ranges[place % C] = [lo, hi) (``BPE.id_ranges``), divided by their mass there (a mass
+    that is 1 but for the type's rounding changes nothing): what lies outside is not read, and need not be 0.  So the ids kept and drawn are distributed as the target held to the range,
+    whether the drafts were drawn from the whole row or inside the range: one outside is passed over, as is every child
+    of a draft row without mass inside."""
     return Verified(*(_bound or _ops()).verify(parents, ids, target, draft, u, ranges, start))
 
 

@@ -19,6 +19,277 @@ from test_draft import (_ATTEND, _Vocabulary, attend, check_attention, check_ver
 BF, FP = torch.bfloat16, torch.float16
 
 
+# ---------------------------------------------------------------- rows held to their place's ids
+def ref_held(parents, ids, target, draft_, u, ranges, start):
+    """Verification with ranges: every row divided by what it holds inside the range of its place (1 where that is 1 but for
+    the type's rounding, half a step and 2^-20 for a 32-bit softmax's sum), drafted ids outside it (or of a draft row without
+    mass there) passed over.  64 bits, a loop over the children."""
+    near = torch.finfo(target.dtype).eps / 2 + 2.0 ** -20
+    mass = lambda x: 1.0 if abs(x.sum() - 1) <= near else x.sum()  # noqa: E731
+    ids, u, parents, start = ids.cpu().numpy(), u.double().cpu().numpy(), parents.cpu().numpy(), start.cpu().numpy()
+    ranges = ranges.cpu().numpy()
+    B, N, V = target.shape
+    clean = lambda x: np.where(np.isfinite(x) & (x > 0), x, 0.0)  # noqa: E731
+    target = clean(target.double().cpu().numpy())
+    draft_ = None if draft_ is None else clean(draft_.double().cpu().numpy())
+    n, paths, tokens = np.zeros(B, int), np.full((B, N), -1), np.full((B, N), -1)
+    for b in range(B):
+        par = (parents if parents.ndim == 1 else parents[b]).tolist()
+        present = tree_paths(par)
+        if present[0] is None:
+            continue
+        path, toks = [0], []
+        while True:
+            c = path[-1]
+            lo, hi = ranges[(int(start[b]) + len(toks)) % len(ranges)]
+            lo, hi = max(int(lo), 0), min(int(hi), V)
+            p = target[b, c, lo:hi] if lo < hi else np.zeros(0)
+            r, Z, kept = p.copy(), mass(p), None
+            if draft_ is not None:
+                q = draft_[b, c, lo:hi] if lo < hi else np.zeros(0)
+                Q = mass(q)
+            for i in range(c + 1, N):
+                x = int(ids[b, i]) - lo
+                if present[i] is None or par[i] != c or not 0 <= x < hi - lo:
+                    continue
+                if draft_ is None:
+                    took, most = np.zeros(hi - lo), Z
+                    took[x] = np.inf
+                elif Q > 0:
+                    took, most = q * (Z / Q), q[x] * (Z / Q)
+                else:
+                    continue
+                if u[b, i] * most < r[x]:
+                    kept = i
+                    break
+                r = np.maximum(r - took, 0.0)
+                Z = r.sum()
+            if kept is None:
+                break
+            path.append(kept)
+            toks.append(int(ids[b, kept]))
+        if not r.sum() > 0:
+            r = p
+        cum = np.cumsum(r)
+        if len(cum) and cum[-1] > 0:
+            hit = np.flatnonzero(cum > u[b, 0] * cum[-1])
+            toks.append(lo + (int(hit[0]) if len(hit) else int(np.flatnonzero(r)[-1])))
+        else:
+            toks.append(-1)
+        n[b] = len(path)
+        paths[b, :len(path)] = path
+        tokens[b, :len(toks)] = toks
+    return n, paths, tokens
+
+
+def make_held(seed, B, N, V, dtype, kind, ranges, drafted=True, sharp=2.0):
+    """Rows over the whole vocabulary, ids drawn from them: some outside their range."""
+    c = make_verify(seed, B, N, V, dtype, kind, True, sharp)
+    g = np.random.default_rng(seed + 1000)
+    c["ranges"] = torch.tensor(ranges, dtype=torch.int32)
+    c["start"] = torch.tensor(g.integers(0, 50, B), dtype=torch.int32)
+    for b in range(B):  # (a range of a few ids seldom meets an id of the whole vocabulary)
+        for i, path in enumerate(tree_paths(c["parents"][b].tolist())):
+            lo, hi = c["ranges"][(int(c["start"][b]) + len(path) - 2) % len(ranges)].clamp(0, V).tolist()
+            if i and hi > lo and g.random() < 0.7:
+                c["ids"][b, i] = int(g.integers(lo, hi))
+    if not drafted:
+        c["draft"] = None
+    return c
+
+
+FIRST = [  # ids, range, drafted: tokens after a root with three drafts of its own
+    (12, (3, 9), True), (12, (3, 9), False), (12, (0, 12), True), (300, (7, 12), True), (300, (7, 12), False),
+]
+
+
+def first_tokens(V, held, drafted, B, seed):
+    """One root, three drafts drawn from its draft row, the rows' mass in and outside the range [lo, hi)."""
+    g = torch.Generator().manual_seed(seed)
+    p = torch.softmax(torch.randn(V, generator=g) * 1.5, -1)
+    q = torch.softmax(torch.randn(V, generator=g) * 1.5, -1)
+    lo, hi = held
+    inside = torch.zeros(V, dtype=torch.bool)
+    inside[lo:hi] = True
+    if not inside.all():  # (half of the target's mass and a third of the draft's lie outside)
+        p, q = (torch.where(inside, a * x / x[inside].sum(), (1 - a) * x / x[~inside].sum()) for x, a in ((p, 1 / 2), (q, 2 / 3)))
+    N = 4
+    ids = torch.multinomial(q.expand(B, V), N, replacement=True, generator=g)
+    if not drafted:  # (the same ids for everyone, the likeliest first: what is kept of them too often shows)
+        ids = (lo + p[lo:hi].topk(N).indices).expand(B, N).contiguous()
+    c = dict(parents=torch.tensor([-1, 0, 0, 0], dtype=torch.int32), ids=ids, target=p.expand(B, N, V),
+             draft=q.expand(B, N, V) if drafted else None, u=torch.rand(B, N, generator=g),
+             ranges=torch.tensor([held], dtype=torch.int32), start=torch.zeros(B, dtype=torch.int32))
+    want = p.double()[lo:hi] / p.double()[lo:hi].sum()
+    return c, want
+
+
+def share_of_target(tokens, held, want):
+    """Every id's share within 5 standard deviations of the target's row held to the range."""
+    lo, hi = held
+    assert ((tokens >= lo) & (tokens < hi)).all()
+    share = torch.bincount(tokens - lo, minlength=hi - lo).double() / len(tokens)
+    return bool(((share - want).abs() <= 5 * (want * (1 - want) / len(tokens)).sqrt()).all())
+
+
+@pytest.mark.parametrize("V,held,drafted", FIRST)
+def test_held_rows_follow_the_target_plainly(V, held, drafted):
+    """The plain implementation itself: the target's row divided by its mass in the range.  Rows taken as they are
+    inside it (their mass as 1) give other shares wherever mass lies outside."""
+    c, want = first_tokens(V, held, drafted, 2048, 3)
+    args = [c[k] for k in ("parents", "ids", "target", "draft", "u", "ranges", "start")]
+    assert share_of_target(torch.tensor(ref_held(*args)[2][:, 0]), held, want)
+    as_they_are = torch.tensor(ref_verify(*args)[2][:, 0])
+    assert share_of_target(as_they_are, held, want) == (held == (0, V))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("V,held,drafted", FIRST)
+def test_verify_held_rows_follow_the_target(V, held, drafted, dtype):
+    c, want = first_tokens(V, held, drafted, 8192, 5)
+    if dtype == BF:  # (a row in 16 bits is another row: its own shares are the ones to follow)
+        c["target"] = c["target"][:1, :1].to(BF).expand_as(c["target"])
+        lo, hi = held
+        want = c["target"][0, 0, lo:hi].double()
+        want = want / want.sum()
+        if drafted:
+            c["draft"] = c["draft"][:1, :1].to(BF).expand_as(c["draft"])
+    r = verify(on(c))
+    assert share_of_target(r.tokens[:, 0].cpu().long(), held, want)
+    assert int((r.n == 2).sum()) > 500
+
+
+HELD = [
+    # B, N, V, tree, ranges
+    (9, 20, 300, "random", [[0, 285], [290, 295], [295, 300], [285, 290]]),
+    (6, 30, 60, "flat", [[10, 50]]),
+    (6, 30, 60, "flat", [[3, 8], [5, 60]]),
+    (12, 7, 1091, "chain", [[0, 1076], [1081, 1086], [1086, 1091], [1076, 1081]]),
+    (5, 128, 90, "random", [[0, 17], [17, 34], [34, 90]]),
+    (4, 128, 50, "flat", [[1, 49]]),
+    (5, 9, 5123, "random", [[0, 5108], [5108, 5123]]),
+    (3, 6, 20001, "flat", [[1, 20000], [19000, 30000]]),
+    (3, 4, 70001, "random", [[-5, 69999], [5, 70001], [0, 40000]]),
+    (2, 1, 40, "chain", [[5, 9]]),
+    (4, 6, 40, "random", [[0, 0], [10, 5], [50, 60], [0, 40]]),
+    (4, 6, 40, "random", [[7, 8], [0, 40]]),
+    (3, 65, 200, "random", [[0, 64], [64, 129], [100, 116], [100, 117]]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafted", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, BF, FP])
+@pytest.mark.parametrize("shape", HELD, ids=lambda s: "x".join(map(str, s[:4])))
+def test_verify_held_rows(shape, dtype, drafted):
+    B, N, V, kind, ranges = shape
+    c = make_held(31, B, N, V, dtype, kind, ranges, drafted)
+    want = ref_held(c["parents"], c["ids"], c["target"], c["draft"], c["u"], c["ranges"], c["start"])
+    check_verify(verify(on(c)), want)
+    d = on(c)  # int32 ids, rows that begin anywhere
+    d["ids"] = d["ids"].int()
+    wide = torch.full((B, N, V + 9), float("nan"), dtype=dtype, device="cuda")
+    wide[..., 3:V + 3] = d["target"]
+    d["target"] = wide[..., 3:V + 3]
+    check_verify(verify(d), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafted", [True, False])
+@pytest.mark.parametrize("V,ranges", [(40, [[3, 30]]), (40, [[3, 12], [20, 25]]), (9000, [[10, 8999]])])
+def test_verify_held_rows_edges(V, ranges, drafted):
+    """Rows and drafts without mass in the range, rows of any mass, equal rows, ids outside the range and the vocabulary, the
+    same id twice, numbers at both ends, absent nodes."""
+    B, N = 14, 10
+    c = make_held(32, B, N, V, torch.float32, "random", ranges, drafted)
+    lo, hi = ranges[0]
+    c["parents"][3:10] = torch.tensor([-1] + [0] * (N - 1), dtype=torch.int32)
+    c["target"][0] = 0
+    c["target"][1, :, lo:hi:2] = float("nan")
+    c["target"][1, :, lo + 1] = float("inf")
+    c["target"][2] *= 1e-30
+    c["target"][4] *= 7
+    c["ids"][5, 1:6] = torch.tensor([-1, V, 2 ** 40, lo - 1, hi])
+    c["ids"][6] = lo + 2
+    c["u"][7] = 0
+    c["u"][8] = float(np.nextafter(np.float32(1), np.float32(0)))
+    c["u"][9] = float("nan")
+    c["parents"][10, 0] = 0
+    c["parents"][11, 1] = -1
+    c["start"][12] = -7
+    c["start"][13] = 2 ** 31 - 1
+    if drafted:
+        c["draft"][3, :, lo:hi] = 0
+        c["draft"][4] = c["target"][4] / 2
+        c["draft"][7] *= 1e30
+        c["draft"][8, :, lo + 1:hi:3] = 0
+    want = ref_held(c["parents"], c["ids"], c["target"], c["draft"], c["u"], c["ranges"], c["start"])
+    assert want[0][10] == 0 and want[2][0, 0] == -1
+    check_verify(verify(on(c)), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafted", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, BF, FP])
+@pytest.mark.parametrize("V", [40, 1091, 20001])
+def test_verify_ranges_that_leave_nothing_out(V, dtype, drafted):
+    """Rows that sum to 1 but for their rounding inside the range are used as they are: a range of everything, or of all that
+    is not 0, changes no id."""
+    c = make_verify(34, 64, 9, V, dtype, "random", drafted)
+    want = ref_verify(c["parents"], c["ids"], c["target"], c["draft"], c["u"])
+    d = on(c)
+    check_verify(verify(d), want)
+    d["ranges"], d["start"] = torch.tensor([[0, V], [-1, V + 3]], dtype=torch.int32).cuda(), torch.arange(64, dtype=torch.int32).cuda()
+    check_verify(verify(d), want)
+    ranges = torch.tensor([[0, V - 15], [V - 10, V - 5], [V - 5, V], [V - 15, V - 10]], dtype=torch.int32)
+    c = make_verify(35, 64, 9, V, dtype, "random", drafted, ranges=ranges)
+    check_verify(verify(on(c)), ref_verify(c["parents"], c["ids"], c["target"], c["draft"], c["u"], ranges, c["start"]))
+
+
+@pytest.mark.gpu
+def test_verify_held_rows_captured():
+    """A captured call with ranges, replayed over new rows and numbers with eager calls between."""
+    ranges = [[0, 285], [290, 295], [295, 300], [285, 290]]
+    c = make_held(33, 6, 20, 300, torch.float32, "random", ranges)
+    d = on(c)
+    verify(d)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = verify(d)
+    for seed in range(4):
+        c = make_held(40 + seed, 6, 20, 300, torch.float32, "random", ranges)
+        for k in d:
+            d[k].copy_(c[k])
+        g.replay()
+        want = ref_held(c["parents"], c["ids"], c["target"], c["draft"], c["u"], c["ranges"], c["start"])
+        check_verify(out, want)
+        check_verify(verify(d), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafted", [True, False])
+def test_vocabulary_holds_plain_rows_to_their_place(drafted):
+    """BPE.verify_draft over a model's plain softmax, wider than the vocabulary: the first token after the root is
+    distributed as the target's row among the ids of its place."""
+    v = _Vocabulary()
+    V, B, N = v.vocab_size + 3, 8192, 4
+    g = torch.Generator().manual_seed(8)
+    for place in range(4):
+        p = torch.softmax(torch.randn(V, generator=g), -1)
+        q = torch.softmax(torch.randn(V, generator=g), -1)
+        ids = torch.multinomial(q.expand(B, V), N, replacement=True, generator=g)
+        u = torch.rand(B, N, generator=g)
+        lo, hi = v.id_ranges()[place].tolist()
+        if not drafted:
+            ids = (lo + p[lo:hi].topk(3).indices[[0, 0, 1, 2]]).expand(B, N).contiguous()
+        r = v.verify_draft(torch.tensor([-1, 0, 0, 0], dtype=torch.int32).cuda(), ids.cuda(), p.cuda().expand(B, N, V),
+                           q.cuda().expand(B, N, V) if drafted else None, u.cuda(),
+                           torch.full((B,), 4 * 9 + place, dtype=torch.int32).cuda())
+        want = p.double()[lo:hi] / p.double()[lo:hi].sum()
+        assert share_of_target(r.tokens[:, 0].cpu().long(), (lo, hi), want)
+
+
 # ---------------------------------------------------------------- flags of a tree's tiles
 def test_a_tiles_flag_is_its_own(tmp_path):
     """csrc/draft.h's flags of tiles with values that are not finite, in the order that waves may take: one has gone on to the
