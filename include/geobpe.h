@@ -356,7 +356,7 @@ int geobpe_run_exchange_log(geobpe_ctx *ctx, int64_t n_merges, int64_t *n_done, 
  * default stream); nothing is allocated or waited for.  Strides are in elements (commit: bytes)
  * and may be any multiple of 16 bytes where rows of a head are meant (the attention's page and
  * slot strides from 0 to below 64 GiB).  A table's positions, max_pages page_size, are at most
- * 2^31 - 4096.  GEOBPE_EARG: sizes, alignment or a null pointer; the message is in
+ * 2^31 - 4096.  GEOBPE_EARG: sizes, alignment, a null pointer or a scale beyond +-2e38; the message is in
  * geobpe_draft_error() (of this thread). */
 typedef struct {
   const void *d_q, *d_k_cache, *d_v_cache, *d_k, *d_v; /* queries; pages; the nodes' own keys and values */

@@ -1,6 +1,7 @@
 // draft.hip -- C entries of the decoding operators (include/geobpe.h, "decoding"): device pointers,
 // the caller's stream, no allocation and no synchronisation, so every call can be captured.
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -206,7 +207,9 @@ int geobpe_tree_attention(int device, void* stream, const geobpe_attend_args* p,
   const geobpe_attend_args& x = *p;
   AttendPlan plan;
   const int rc = attend_sizes(x, plan);
-  if (rc != GEOBPE_OK || x.seqs == 0) return rc;
+  if (rc != GEOBPE_OK) return rc;
+  if (!(fabs(x.scale) <= 2e38)) return fail(GEOBPE_EARG, "tree attention: scale %g is not finite in 32 bits", x.scale);
+  if (x.seqs == 0) return GEOBPE_OK;
   if (!x.d_q || !x.d_k_cache || !x.d_v_cache || !x.d_k || !x.d_v || !x.d_lens || !x.d_parents || !x.d_out ||
       (x.max_pages && !x.d_table) || (plan.bytes && !d_work))
     return fail(GEOBPE_EARG, "tree attention: null pointer");

@@ -26,6 +26,7 @@ struct {
 PyObject* geobpe_error;  // geobpe._native.GeoBPEError
 
 constexpr int64_t MAX_NODES = 128, MAX_VOCAB = 1 << 22, MAX_POSITIONS = 0x7ffff000;
+constexpr double MAX_SCALE = 2e38;  // times log2 e it is one of float32's finite numbers
 
 struct Refused {};  // thrown with the Python error set
 
@@ -217,6 +218,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* o, Py_ssize_t nargs) {
   if (o[8] != Py_None) {
     scale = PyFloat_AsDouble(o[8]);
     if (scale == -1.0 && PyErr_Occurred()) throw Refused();
+    if (!(std::fabs(scale) <= MAX_SCALE)) VALUE("scale %R: a finite number up to 2e38 in size is expected", o[8]);
   }
   no_grad({&q, c.k, c.v, &k, &v});
   geobpe_attend_args a;

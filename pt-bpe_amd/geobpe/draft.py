@@ -64,7 +64,8 @@ def tree_attention(q, k_cache, v_cache, block_table, lens, k, v, parents, scale:
     multiple of 8 up to 256, Hq a multiple of Hkv (query head h reads kv head h // (Hq // Hkv)).
     k_cache, v_cache (pages, page size, Hkv, D): position x of sequence b is slot x % page size of page
     block_table[b, x // page size]; lens (B,): its committed positions.  Other orders of the cache's
-    dimensions are views with strides (16-byte aligned rows).  scale: D ** -0.5 if None.  A call has at most
+    dimensions are views with strides (16-byte aligned rows).  scale: D ** -0.5 if None, else a
+    finite number up to 2e38 in size.  A call has at most
     2^23 - 1 query rows (B N Hq) and a table MAX_POSITIONS positions.
 
     Returns (B, N, Hq, D).  Rows of absent nodes are 0 whatever their keys and values hold, and so does

@@ -340,3 +340,17 @@ def test_attention_values_not_finite_by_tile(N, Hq, D, where):
     d = on(c)
     for _ in range(3):
         check_attention(attend(d), want, BF)
+
+
+# ---------------------------------------------------------------- scales and scores
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39, -1e300, 3e38])
+def test_attention_refuses_scales_that_are_not_finite(scale):
+    """NaN, infinities and what is none of float32's: a call would answer with a plain mean, or with NaN."""
+    from geobpe import _native
+    c = make_attention(0, 2, 3, [5, 9], 4, 2, 16, 4, BF)
+    refuse(attend, c, ValueError, "scale", scale=scale)
+    refuse(attend, c, TypeError, "real number|float", scale="1")
+    L = _native.lib()
+    args = ([256] * 9 + [64] * 15 + [1, 0] + [1, 2, 4, 2, 64, 16, 3, 2, 0])
+    assert L.geobpe_tree_attention(0, None, _ATTEND.pack(*args, scale), 256, 1 << 40) == _native.E_ARG
+    assert b"scale" in L.geobpe_draft_error()
