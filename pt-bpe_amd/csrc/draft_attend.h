@@ -78,9 +78,9 @@ __device__ inline uint64_t pack4(f32x4 v) {
 }
 
 // Scores are compared as q k and scaled inside the exponent's multiply-add, exp2(q k c - max c), c = |scale| log2 e; a
-// negative scale turns the queries' signs.  A scale of 0 leaves a c that is too small to matter: -inf, what is not
-// there, stays -inf.
-__device__ inline float score_scale(float scale) { return fmaxf(fabsf(scale) * LOG2E, 1e-30f); }
+// negative scale turns the queries' signs.  A scale of 0 leaves float32's smallest c, which takes no score to more than
+// 2^-21 (with 1e-30 products of 1e30 and more were scores still): -inf, what is not there, stays -inf.
+__device__ inline float score_scale(float scale) { return fmaxf(fabsf(scale) * LOG2E, 0x1p-149f); }
 __device__ inline u32x4 negative(u32x4 q) { return q ^ u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u}; }
 // a row that has seen no key has the maximum -inf: its weights are taken from 0, and are 0
 __device__ inline float at_least(float mx) { return mx == -INFINITY ? 0.f : mx; }

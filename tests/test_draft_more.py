@@ -354,3 +354,17 @@ def test_attention_refuses_scales_that_are_not_finite(scale):
     args = ([256] * 9 + [64] * 15 + [1, 0] + [1, 2, 4, 2, 64, 16, 3, 2, 0])
     assert L.geobpe_tree_attention(0, None, _ATTEND.pack(*args, scale), 256, 1 << 40) == _native.E_ARG
     assert b"scale" in L.geobpe_draft_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [3, 40])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-33, -1e-33, 1e-38, 1e-45])
+def test_attention_small_scales_of_large_scores(N, scale):
+    """Products q k of up to 1e33: a scale of 0 is the mean of the values all the same, and one of 1e-33 gives scores of
+    some units."""
+    c = make_attention(51, 2, N, [90, 600], 4, 2, 16, 16, BF)
+    c["q"] = (c["q"].float() * 1e16).to(BF)
+    c["k"] = (c["k"].float() * 1e16).to(BF)
+    c["k_cache"] = (c["k_cache"].float() * 1e16).to(BF)
+    c["scale"] = scale
+    check_attention(attend(on(c)), ref_attention(**c), BF)
