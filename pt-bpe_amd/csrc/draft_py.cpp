@@ -3,7 +3,7 @@
 // than the kernels of small calls.  The entries of libgeobpe.so are bound by address (geobpe._native has loaded it), so
 // this module needs the process's PyTorch and nothing else.
 #include <ATen/ops/empty.h>
-#include <c10/core/GradMode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -118,10 +118,16 @@ hipStream_t stream_of(at::Device device) {
   return c10::hip::getCurrentHIPStream(device.index()).stream();
 }
 
+// no derivatives: neither backward nor forward ones, which no_grad() leaves on
 void no_grad(std::initializer_list<const at::Tensor*> xs) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (const at::Tensor* x : xs)
-    if (x && x->requires_grad()) VALUE("the decoding operators have no backward: call them under torch.no_grad()");
+  const c10::AutogradState& now = c10::AutogradState::get_tls_state();
+  for (const at::Tensor* x : xs) {
+    if (!x) continue;
+    if (now.get_grad_mode() && x->requires_grad())
+      VALUE("the decoding operators have no backward: call them under torch.no_grad()");
+    if (now.get_fw_grad_mode() && x->_fw_grad(0).defined())
+      VALUE("the decoding operators have no backward and take no tangents: call them on the primal tensors");
+  }
 }
 
 void nodes(int64_t N) {

@@ -13,7 +13,8 @@ tree or (batch, N).
 
 The tensors are torch tensors of one device.  Calls are ordered on the current stream of that device,
 wait for nothing, take their outputs from torch's allocator and can be captured.  There is no
-CPU fallback and no backward: inputs that require gradients are refused unless gradients are off.
+CPU fallback and no backward: inputs that require gradients are refused unless gradients are off, and so are
+inputs with tangents (forward mode) outside inference mode.
 """
 from __future__ import annotations
 

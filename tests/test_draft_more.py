@@ -368,3 +368,22 @@ def test_attention_small_scales_of_large_scores(N, scale):
     c["k_cache"] = (c["k_cache"].float() * 1e16).to(BF)
     c["scale"] = scale
     check_attention(attend(on(c)), ref_attention(**c), BF)
+
+
+# ---------------------------------------------------------------- what autograd is told
+def test_tangents_are_refused():
+    """There is no forward derivative either: a tensor with a tangent would lose it without a word."""
+    import torch.autograd.forward_ad as fw
+    a, v, k = (make_attention(0, 2, 3, [5, 9], 4, 2, 16, 4, BF), make_verify(0, 2, 4, 20, torch.float32, "random"),
+               make_commit(0, 2, 3, 4, [0, 5, 7], 2, 16, 4, BF))
+    with fw.dual_level():
+        for f, c, names in ((attend, a, ("q", "k_cache", "v_cache", "k", "v")), (verify, v, ("target", "draft")),
+                            (commit, k, ("k_cache", "v_cache", "k", "v"))):
+            for name in names:
+                dual = fw.make_dual(c[name], torch.ones_like(c[name]))
+                refuse(f, c, ValueError, "no backward", **{name: dual})
+                with torch.no_grad():  # (tangents go on under no_grad)
+                    refuse(f, c, ValueError, "no backward", **{name: dual})
+                with torch.inference_mode():
+                    refuse(f, c, ValueError, "HIP device only", **{name: dual})
+            refuse(f, c, ValueError, "HIP device only")
