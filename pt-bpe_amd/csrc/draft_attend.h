@@ -35,6 +35,8 @@ constexpr int ATT_TILE = 32;  // keys a wave works on at a time
 // / 2048 workgroups 64 chains of 5 nodes over up to 2237 positions took 42 / 49 / 44 us when they were cut at all), but no
 // part gets below 16 tiles (with 8 one token over 237 positions took 10.8 us instead of 8.2).
 constexpr int ATT_WANT = 512, ATT_LEAST = 16;
+// a part's sum of an absent row: a present one's is 0 when all of its scores are -infinity, and its result is 0 / 0 then
+constexpr float PART_ABSENT = -1.f;
 constexpr float LOG2E = 1.44269504088896340736f;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -501,12 +503,12 @@ __global__ __launch_bounds__(64 * W, KS <= 4 ? 2 : 1) void k_attend(AttendArgs a
         *(uint64_t*)out = here ? pack4<T>(acc * (1.f / total)) : 0;
       } else {
         const int64_t at = part_row(a, rt, item, part, RB * 16, r * 16 + row);
-        const f32x4 none = {0.f, 0.f, 0.f, 0.f};  // an absent row's parts: a sum of 0
+        const f32x4 none = {0.f, 0.f, 0.f, 0.f};
         *(f32x4*)(a.part + at * a.D + d) = here ? acc : none;
         if (d == 0) {
           float* p = part_sums(a, a.row_tiles, RB * 16) + 2 * at;
           p[0] = here ? mx : -INFINITY;
-          p[1] = here ? total : 0.f;
+          p[1] = here ? total : PART_ABSENT;
         }
       }
     }
@@ -981,14 +983,14 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_atte
       if (sh.parts > 1 && hh == 0) {
         float* ml = part_sums(a, a.row_tiles, ROWS) + 2 * at;
         ml[0] = here ? top : -INFINITY;
-        ml[1] = here ? sum : 0.f;
+        ml[1] = here ? sum : PART_ABSENT;
       }
       for (int d = 0; d < DB; d++)
         for (int i = 0; i < 4; i++) {
           const int x = 32 * d + 8 * i + 4 * hh;
           if (x >= a.D) continue;
           const f32x4 y = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}, none = {0.f, 0.f, 0.f, 0.f};
-          if (sh.parts > 1)  // (an absent row's parts: a sum of 0)
+          if (sh.parts > 1)
             *(f32x4*)(a.part + at * a.D + x) = here ? y : none;
           else
             *(uint64_t*)(lds + own + (l32 * CH + key_slot<CH>(l32, 4 * d + i)) * 16 + 8 * hh) = here ? pack4<T>(y * f) : 0;
@@ -1055,8 +1057,9 @@ __global__ __launch_bounds__(ATT_BLOCK) void k_attend_join(AttendArgs a, int row
     for (int k = 1; k < BY; k++) add(ml_[0][t + k * q], ml_[1][t + k * q], acc_[t + k * q]);
   }
   if (parts == 1) return;
+  const bool absent = ml[2 * base + 1] == PART_ABSENT;
   T* out = (T*)a.out + (((int64_t)b * a.N + n) * a.Hq + h * G + m - n * G) * a.D + d;
-  *(uint64_t*)out = total == 0.f ? 0 : pack4<T>(acc * (1.f / total));
+  *(uint64_t*)out = absent ? 0 : pack4<T>(acc * (1.f / total));
 }
 
 }  // namespace gb

@@ -387,3 +387,20 @@ def test_tangents_are_refused():
                 with torch.inference_mode():
                     refuse(f, c, ValueError, "HIP device only", **{name: dual})
             refuse(f, c, ValueError, "HIP device only")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,lens", [(3, [40, 5000, 0]), (40, [40, 5000, 0]), (40, [5000, 5000, 5000])])
+def test_attention_rows_without_weights(N, lens):
+    """A present node all of whose scores are -infinity has no weights: NaN, whether its sequence is cut into parts or not.
+    An absent node's row stays 0."""
+    c = make_attention(61, 3, N, lens, 2, 1, 64, 16, BF)
+    used = ~torch.isnan(c["k_cache"])
+    c["k_cache"][..., 0] = torch.where(used[..., 0], -1.0, float("nan")).to(BF)
+    c["k"][..., 0] = -1
+    c["q"][:, 1, 1, 0] = float("inf")
+    c["q"][:, N - 1, 0, 0] = float("inf")
+    c["parents"][:, N - 1] = -3
+    want = ref_attention(**c)
+    assert np.isnan(want[0][:, 1, 1]).all() and not want[0][:, N - 1].any() and np.isfinite(want[0][:, 0]).all()
+    check_attention(attend(on(c)), want, BF)
