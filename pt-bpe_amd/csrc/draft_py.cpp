@@ -342,6 +342,8 @@ PyObject* commit(PyObject*, PyObject* const* o, Py_ssize_t nargs) {
   a.layers = L, a.seqs = c.B, a.nodes = N, a.kv_heads = c.Hkv, a.head_bytes = c.D * e;
   a.page_size = c.S, a.pages = c.P, a.max_pages = c.M;
   called(lib.commit(dev.index(), stream, &a));
+  for (const at::Tensor* x : {c.k, c.v})  // they were written: a backward pass that needs them as they were has to see it
+    if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
   return THPVariable_Wrap(std::move(out));
   END_GUARDED
 }

@@ -404,3 +404,19 @@ def test_attention_rows_without_weights(N, lens):
     want = ref_attention(**c)
     assert np.isnan(want[0][:, 1, 1]).all() and not want[0][:, N - 1].any() and np.isfinite(want[0][:, 0]).all()
     check_attention(attend(on(c)), want, BF)
+
+
+@pytest.mark.gpu
+def test_commit_tells_autograd_of_its_writes():
+    """A cache that a later backward pass needs as it was: torch has to see that it was written."""
+    c = on(make_commit(71, 2, 3, 4, [0, 5, 7], 2, 16, 4, torch.float32))
+    before = c["k_cache"]._version, c["v_cache"]._version
+    w = torch.ones(16, device="cuda", requires_grad=True)
+    y = (c["k_cache"] * w).sum() + (c["v_cache"] * w).sum()
+    commit(c)
+    assert c["k_cache"]._version > before[0] and c["v_cache"]._version > before[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():  # (tensors without a version)
+        d = {k: v.clone() for k, v in c.items()}
+        assert torch.equal(commit(d), commit({**c, "k_cache": c["k_cache"].clone(), "v_cache": c["v_cache"].clone()}))
