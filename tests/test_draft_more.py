@@ -420,3 +420,116 @@ def test_commit_tells_autograd_of_its_writes():
     with torch.inference_mode():  # (tensors without a version)
         d = {k: v.clone() for k, v in c.items()}
         assert torch.equal(commit(d), commit({**c, "k_cache": c["k_cache"].clone(), "v_cache": c["v_cache"].clone()}))
+
+
+# ---------------------------------------------------------------- long contexts, every tile visible
+def level(L):
+    """A position's score in powers of two: parts of 512 positions lie up to 2^12 apart."""
+    return (np.arange(L) // 512 * 5) % 13 - 6
+
+
+def make_visible(seed, N, L, G, Hkv, D, dtype, S=64):
+    """One sequence of L positions and a chain of N nodes.  Position x's weight is nearly 2^level.  Marked positions have the value
+    2^-level in one channel and 0 in the others, so that a channel of a result is the sum of a few shares that are about alike:
+    the first half of the kv heads has a channel for every 512 positions, the second one for the ends of every 16 (about
+    L / (4 Hkv D) of them a channel).  The level also is channel 0 of the keys."""
+    g = np.random.default_rng(seed)
+    M = -(-L // S)
+    x, pages, half = np.arange(L), g.permutation(M + 1)[:M], Hkv // 2
+    k = g.standard_normal((L, Hkv, D)) * 0.25
+    k[:, :, 0] = level(L)[:, None]
+    v = np.zeros((L, Hkv, D))
+    v[x, x // 512 % half, x // 512 // half % D] = 2.0 ** -level(L)
+    ends = x[(x % 16 == 0) | (x % 16 == 15) | (x == L - 1)]
+    turn = ends // 16 * 2 + (ends % 16 > 0)
+    v[ends, half + turn % half, turn // half % D] = 2.0 ** -level(L)[ends]
+    kc, vc = (torch.full((M + 1, S, Hkv, D), float("nan"), dtype=dtype) for _ in range(2))
+    page = torch.tensor(pages[x // S])
+    kc[page, x % S], vc[page, x % S] = torch.tensor(k).to(dtype), torch.tensor(v).to(dtype)
+    q = g.standard_normal((1, N, Hkv * G, D)) * 0.25
+    q[..., 0] = np.log(2) * D ** 0.5
+    own = g.standard_normal((1, N, Hkv, D)) * 0.25
+    own[..., 0] = 0
+    t = lambda y: torch.tensor(y).to(dtype)  # noqa: E731
+    return dict(q=t(q), k_cache=kc, v_cache=vc, block_table=torch.tensor(pages[None], dtype=torch.int32),
+                lens=torch.tensor([L], dtype=torch.int32), k=t(own), v=t(np.zeros((1, N, Hkv, D))),
+                parents=torch.arange(-1, N - 1, dtype=torch.int32))
+
+
+def visible_heads(c):
+    """Per query head the weights (nodes x keys) and the values (keys x D), float64, of one sequence whose nodes are a chain."""
+    L, S = int(c["lens"][0]), c["k_cache"].shape[1]
+    x = np.arange(L)
+    page = c["block_table"][0].long().numpy()[x // S]
+    kc, vc = c["k_cache"].double().numpy()[page, x % S], c["v_cache"].double().numpy()[page, x % S]
+    q, k, v = (c[n][0].double().numpy() for n in ("q", "k", "v"))
+    N, Hq, D = q.shape
+    chain = np.tril(np.ones((N, N), bool))
+    for h in range(Hq):
+        g = h // (Hq // k.shape[1])
+        s = np.concatenate([q[:, h] @ kc[:, g].T, np.where(chain, q[:, h] @ k[:, g].T, -np.inf)], 1) * D ** -0.5
+        yield np.exp(s - s.max(1, keepdims=True)), np.concatenate([vc[:, g], v[:, g]])
+
+
+def ref_visible(heads, factor=1.0):
+    """The result and sum w |v| / sum w, the cache's weights multiplied by ``factor`` (0: a lost key)."""
+    out, mag = [], []
+    for w, v in heads:
+        w = w.copy()
+        w[:, :w.shape[1] - w.shape[0]] *= factor
+        out.append(w @ v / w.sum(1, keepdims=True))
+        mag.append(w @ np.abs(v) / w.sum(1, keepdims=True))
+    return np.stack(out, 1)[None], np.stack(mag, 1)[None]
+
+
+VISIBLE = [  # nodes, positions, query heads a kv head, kv heads, head
+    (2, 70001, 1, 8, 128), (5, 5000, 2, 4, 64), (1, 40000, 4, 8, 96), (16, 70001, 4, 8, 128), (40, 20001, 1, 8, 64),
+    (100, 9000, 2, 4, 128), (3, 12345, 1, 8, 200), (20, 12345, 1, 8, 256),
+]
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("L", [5000, 70001])
+def test_a_lost_tile_would_be_seen(L, dtype):
+    """The check passes for the result rounded to the type, and fails for one without a key at a tile's end, a tile, a part or
+    the last position, and for one whose parts are joined with a weight a little off."""
+    heads = list(visible_heads(make_visible(81, 1, L, 1, 8, 128, dtype)))
+    want, x = ref_visible(heads), np.arange(L)
+    check_attention(torch.tensor(want[0]).to(dtype), want, dtype)
+
+    def seen(which, factor=0.0):
+        got = torch.tensor(ref_visible(heads, np.where(which, factor, 1.0))[0]).to(dtype)
+        try:
+            check_attention(got, want, dtype)
+        except AssertionError:
+            return True
+        return False
+
+    for at in (0, 31, 32, 511, 512, 2047, 2048, L // 32 * 32, L - 1):
+        assert seen(x == at) and seen((x >= at) & (x < at + 32)), at
+    part = x // 512 == 3
+    assert seen(part) and seen(part, 1.05) and seen(x // 512 == x[-1] // 512, 0.95) and not seen(part, 1.0)
+    if L > 10000:
+        assert seen((x >= 20000) & (x < 27000))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("shape", VISIBLE, ids=lambda s: "x".join(map(str, s)))
+def test_attention_of_every_tile(shape, dtype):
+    N, L, G, Hkv, D = shape
+    c = make_visible(82, N, L, G, Hkv, D, dtype)
+    check_attention(attend(on(c)), ref_visible(visible_heads(c)), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [2, 30])
+@pytest.mark.parametrize("N", [2, 40])
+def test_attention_of_every_tile_with_room_in_the_table(N, room):
+    """The parts are cut for the table's positions: the same sequence under a table of ``room`` times as many."""
+    c = make_visible(83, N, 5000, 1, 8, 64, FP)
+    want = ref_visible(visible_heads(c))
+    table = torch.full((1, c["block_table"].shape[1] * room), -1, dtype=torch.int32)
+    table[:, :c["block_table"].shape[1]] = c["block_table"]
+    c["block_table"] = table
+    check_attention(attend(on(c)), want, FP)
