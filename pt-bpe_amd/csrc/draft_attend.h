@@ -79,7 +79,9 @@ __device__ inline uint64_t pack4(f32x4 v) {
   return (uint64_t)pack2<T>(v[2], v[3]) << 32 | pack2<T>(v[0], v[1]);
 }
 
-// Scores are compared as q k and scaled inside the exponent's multiply-add, exp2(q k c - max c), c = |scale| log2 e; a
+// Scores are compared as q k and scaled inside the exponent's multiply-add, exp2((q k - max) c + bias), c = |scale| log2 e.
+// (One subtraction more than q k c - max c, and not slower: where max c is rounded, past 2^30, the largest weight would
+// be anything but 1, and infinite at last.)  A
 // negative scale turns the queries' signs.  A scale of 0 leaves float32's smallest c, which takes no score to more than
 // 2^-21 (with 1e-30 products of 1e30 and more were scores still): -inf, what is not there, stays -inf.
 __device__ inline float score_scale(float scale) { return fmaxf(fabsf(scale) * LOG2E, 0x1p-149f); }
@@ -407,9 +409,8 @@ __global__ __launch_bounds__(64 * W, KS <= 4 ? 2 : 1) void k_attend(AttendArgs a
         sum[r] *= f;
         for (int d = 0; d < DB; d++) o[d][r] *= f;
       }
-      const float off = fmaf(-from, scale, Half<T>::bias);
       for (int c = 0; c < 2; c++)
-        for (int i = 0; i < 4; i++) s[c][r][i] = __builtin_amdgcn_exp2f(fmaf(s[c][r][i], scale, off));
+        for (int i = 0; i < 4; i++) s[c][r][i] = __builtin_amdgcn_exp2f(fmaf(s[c][r][i] - from, scale, Half<T>::bias));
       sum[r] += ((s[0][r][0] + s[0][r][1]) + (s[0][r][2] + s[0][r][3])) +
                 ((s[1][r][0] + s[1][r][1]) + (s[1][r][2] + s[1][r][3]));
       for (int c = 0; c < 2; c++)
@@ -717,12 +718,12 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_atte
       }
     };
     auto weigh = [&](const f32x16* s, u32x4* p) {
-      const float off = fmaf(-at_least(top), scale, Half<T>::bias);
+      const float from = at_least(top);
       float part[4] = {0.f, 0.f, 0.f, 0.f};
       for (int c = 0; c < 2; c++)
         for (int i = 0; i < 16; i += 2) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[c][i], scale, off));
-          const float y = __builtin_amdgcn_exp2f(fmaf(s[c][i + 1], scale, off));
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[c][i] - from, scale, Half<T>::bias));
+          const float y = __builtin_amdgcn_exp2f(fmaf(s[c][i + 1] - from, scale, Half<T>::bias));
           part[i / 2 % 4] += x + y;
           p[2 * c + i / 8][i / 2 % 4] = pack2<T>(x, y);
         }
@@ -818,7 +819,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_atte
       // exponentials of another step's weights
       auto turn = [&](const f32x16* s, f32x16* n, int t, int buf) {
         const uint32_t vb = buf * TILE_BYTES, kb = vb ^ TILE_BYTES;
-        const float off = fmaf(-at_least(top), scale, Half<T>::bias);
+        const float from = at_least(top);
         float part[2] = {0.f, 0.f};
         u32x4 p[4];
         auto keys = [&](int i) {
@@ -837,8 +838,8 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : DP > 32 ? 2 : 3) void k_atte
         auto expo = [&](int st, int half) {
           for (int e = 0; e < 4; e += 2) {
             const int i = 8 * (st & 1) + 4 * half + e;
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[st / 2][i], scale, off));
-            const float y = __builtin_amdgcn_exp2f(fmaf(s[st / 2][i + 1], scale, off));
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[st / 2][i] - from, scale, Half<T>::bias));
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[st / 2][i + 1] - from, scale, Half<T>::bias));
             part[half] += x + y;
             p[st][2 * half + e / 2] = pack2<T>(x, y);
           }

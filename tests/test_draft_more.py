@@ -357,6 +357,32 @@ def test_attention_refuses_scales_that_are_not_finite(scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("N", [3, 40])
+@pytest.mark.parametrize("scale", [1.0, -1.0, 3.0, 1e5, 1e20, 1e30])
+def test_attention_large_scores(N, scale, dtype):
+    """Scores of up to 1e36 whose weights are known: keys are whole numbers times one vector, so every score is a whole number of
+    steps, exact in float32, and all but the largest are at least one step of 2^10 and more below it.  Keys that share the largest
+    share the row's weight."""
+    c = make_attention(55, 3, N, [90, 700, 5000], 4, 2, 64, 16, dtype)
+    g = np.random.default_rng(55)
+
+    def whole(x):  # one whole number of 0 .. 7 in channels 0 and 1, nothing else
+        y = torch.zeros(x.shape)
+        y[..., 0] = torch.tensor(g.integers(0, 8, x.shape[:-1])).float() * 32
+        y[..., 1] = y[..., 0]
+        return torch.where(torch.isnan(x.float()), x.float(), y).to(dtype)
+
+    c["k_cache"], c["k"] = whole(c["k_cache"]), whole(c["k"])
+    c["q"] = torch.zeros(c["q"].shape).to(dtype)
+    c["q"][..., 0] = 100
+    c["q"][..., 1] = 60
+    c["q"][:, 1::2, :, :2] *= -1
+    c["scale"] = scale
+    check_attention(attend(on(c)), ref_attention(**c), dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("N", [3, 40])
 @pytest.mark.parametrize("scale", [0.0, -0.0, 1e-33, -1e-33, 1e-38, 1e-45])
 def test_attention_small_scales_of_large_scores(N, scale):
