@@ -50,7 +50,9 @@ bool aligned(const void* p, const int64_t* strides, int n, int64_t unit) {
   return true;
 }
 
-// how a call is cut: rows a workgroup works on, tiles of keys a part has at most
+// How a call is cut: rows a workgroup works on, tiles of keys a part has at most.  The host does not know the lengths, so the
+// cut is made for the table's positions: short sequences under a long table make few parts (4 x 8 heads over 8191 of 131072
+// positions 228 + 5 us, over 8191 of 8191 30 + 7; the figures below are of tables that fit the longest sequence).
 struct AttendPlan {
   bool wide;
   int rb, waves, rows, tile, per, most;

@@ -31,9 +31,11 @@ struct AttendArgs {
 
 constexpr int ATT_BLOCK = 256;
 constexpr int ATT_TILE = 32;  // keys a wave works on at a time
-// The keys are cut so that about two workgroups of four waves a CU have work (more parts cost their joining: at 512 / 1024
-// / 2048 workgroups 64 chains of 5 nodes over up to 2237 positions took 42 / 49 / 44 us when they were cut at all), but no
-// part gets below 16 tiles (with 8 one token over 237 positions took 10.8 us instead of 8.2).
+// The keys are cut so that about two workgroups of four waves a CU have work: at 512 / 1024 / 2048 workgroups, the join
+// included, one tree over up to 105k positions (2 heads of 48 rows) takes 22 / 28 / 28 us, 7 trees of 27 nodes over up to 4099
+// 30 / 27 / 27, 2 tokens over 30k to 60k (8 heads) 115 / 97 / 99: none is best for all.  A part may have 16 tiles before there is
+// a second one (with 8 one token over 237 positions takes 8.7 us instead of 6.9, 3 chains of 5 nodes over up to 2000 10.7
+// instead of 11.8); as a sequence's parts are equal, they can have about half of that.
 constexpr int ATT_WANT = 512, ATT_LEAST = 16;
 // a part's sum of an absent row: a present one's is 0 when all of its scores are -infinity, and its result is 0 / 0 then
 constexpr float PART_ABSENT = -1.f;
@@ -81,9 +83,9 @@ __device__ inline uint64_t pack4(f32x4 v) {
 
 // Scores are compared as q k and scaled inside the exponent's multiply-add, exp2((q k - max) c + bias), c = |scale| log2 e.
 // (One subtraction more than q k c - max c, and not slower: where max c is rounded, past 2^30, the largest weight would
-// be anything but 1, and infinite at last.)  A
-// negative scale turns the queries' signs.  A scale of 0 leaves float32's smallest c, which takes no score to more than
-// 2^-21 (with 1e-30 products of 1e30 and more were scores still): -inf, what is not there, stays -inf.
+// be anything but 1, and infinite at last.)  A negative scale turns the queries' signs.  A scale of 0 leaves float32's
+// smallest c, which takes no score to more than 2^-21 (with 1e-30 products of 1e30 and more were scores still): -inf, what
+// is not there, stays -inf.
 __device__ inline float score_scale(float scale) { return fmaxf(fabsf(scale) * LOG2E, 0x1p-149f); }
 __device__ inline u32x4 negative(u32x4 q) { return q ^ u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u}; }
 // a row that has seen no key has the maximum -inf: its weights are taken from 0, and are 0
@@ -524,8 +526,10 @@ __global__ __launch_bounds__(64 * W, KS <= 4 ? 2 : 1) void k_attend(AttendArgs a
 //
 // Up to about 100 rows the cache's bytes bound it: 64 rows of heads of 128 over 131071 positions take 111 us and the
 // join 7, 537 MB at 4.8 TB/s.  Above it is the matrix units: 256 rows, 32 sequences over 8k to 16k: 500 to 550 us, 414
-// GFLOP at 750 to 830 TFLOP/s, where the card lowers its clock (the first launches take 480; no order of the
-// instructions, depth of the loads or priority of the waves made the later ones faster).  Small calls are the way from one
+// GFLOP at 750 to 830 TFLOP/s.  There is one workgroup a CU, so the longest sequence, 1.3 times the mean, sets the time, and over
+// all of it the matrix units are busy for 44 % (58 % while a CU has work): the rest is what does not overlap of the
+// exponentials, waits and bank conflicts, and the clock, which the card lowers (the first launches take 480; no order of
+// the instructions, depth of the loads or priority of the waves made the later ones faster).  Small calls are the way from one
 // load to the next again: 432 rows without a prefix 9.6 us.
 //
 // In LDS a row's 16-byte pieces are permuted so that the operands' reads spread over the banks: eight rows' piece of K in
@@ -552,8 +556,9 @@ template <int CH>
 __device__ inline int value_slot(int row, int c) {  // (its own inverse)
   return c ^ (CH >= 16 ? (row & 3) << 2 : CH == 8 ? (row >> 1 & 1) << 2 : 0);
 }
-// A part has at least 4 tiles (2 heads of 432 rows over 960 positions, at least 16 / 8 / 4 / 2 tiles: 36 / 22 / 18 / 15.5 us;
-// with 2 those over 64 took 13.2 instead of 11.0 for the join).  `Many` tiles: eight for every CU.
+// A part may have 4 tiles before there is a second one (2 heads of 432 rows over 960 positions, with 8 / 4 / 2: 23.4 / 18.4 /
+// 16.6 us; with 2 those over 64 take 15.9 instead of 11.6 for the join), and equal parts about half of that.  `Many` tiles:
+// eight for every CU.
 constexpr int WIDE_TILE = DRAFT_TILE, WIDE_LEAST = 4, WIDE_MANY = 2048;
 constexpr float SLACK = 8.f;
 

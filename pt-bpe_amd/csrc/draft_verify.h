@@ -22,7 +22,7 @@
 // of those with drafted children.  r is worked out anew from the
 // rows and the Z so far whenever it is needed, never stored.  One workgroup does a sequence: a row of 128 k entries takes
 // it about as long as the rows' share of the card's bandwidth once there are 100 sequences: 128 chains of 7 drafts over
-// 131072 fp32 entries take 34 us, 134 MB at 4.0 TB/s.  Small calls are dependent loads: one chain over 1091 ids 5.3 us, 48
+// 131072 fp32 entries take 33 us, 134 MB at 4.0 TB/s.  Small calls are dependent loads: one chain over 1091 ids 5.3 us, 48
 // trees of 40 nodes over 5123 ids held to ranges 18.5 (the longest walk: a sum for every context with children, and one per
 // rejected sibling).
 #pragma once
@@ -45,7 +45,8 @@ struct VerifyArgs {
 };
 
 constexpr int VER_MAX_VOCAB = 1 << 22;
-// up to here four waves do a sequence, above 16 (48 trees of 40 nodes over 5123 ids: 14.0 us with four, 16.7 with 16)
+// up to here four waves do a sequence, above 16 (48 trees of 40 nodes over 5123 ids held to ranges: 18.8 us with four, 21.9
+// with 16; one chain over 1091: 5.3 and 5.8)
 constexpr int VER_SMALL = 8192;
 // a sum that falls below this part of itself by subtraction is taken anew: the rest keeps 33 bits and more
 constexpr double VER_KEEP = 1.0 / (1 << 20);

@@ -67,7 +67,9 @@ def tree_attention(q, k_cache, v_cache, block_table, lens, k, v, parents, scale:
     block_table[b, x // page size]; lens (B,): its committed positions.  Other orders of the cache's
     dimensions are views with strides (16-byte aligned rows).  scale: D ** -0.5 if None, else a
     finite number up to 2e38 in size.  A call has at most
-    2^23 - 1 query rows (B N Hq) and a table MAX_POSITIONS positions.
+    2^23 - 1 query rows (B N Hq) and a table MAX_POSITIONS positions.  The work is cut for the table's positions, whatever
+    the lengths: a table far longer than its sequences costs time (some 6 times at 16 times the length), so pass the part of
+    it that can be in use (``block_table[:, :pages]``).
 
     Returns (B, N, Hq, D).  Rows of absent nodes are 0 whatever their keys and values hold, and so does
     nothing outside a node's own path reach its row.  A length outside the table, or a page outside the cache
@@ -113,7 +115,8 @@ def commit(k_cache, v_cache, block_table, lens, k, v, path, n):
 class DraftCache:
     """The keys and values of ``batch`` sequences of up to ``max_len`` committed positions, every layer's, in pages,
     with their lengths.  A model's step over a drafted tree is, per layer, ``attend`` and, once the ids are verified
-    (``verify``, ``BPE.verify_draft``), one ``keep``; ``lens`` is a device tensor throughout."""
+    (``verify``, ``BPE.verify_draft``), one ``keep``; ``lens`` is a device tensor throughout.  A prompt goes in as chains of
+    up to MAX_NODES nodes, each kept whole: ``keep(k, v, Verified(n, path, None))``, path[b] = 0, 1, ..., n[b] its nodes."""
 
     def __init__(self, layers: int, batch: int, max_len: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16,
                  device="cuda", page_size: int = 64):

@@ -559,3 +559,40 @@ def test_attention_of_every_tile_with_room_in_the_table(N, room):
     table[:, :c["block_table"].shape[1]] = c["block_table"]
     c["block_table"] = table
     check_attention(attend(on(c)), want, FP)
+
+
+# ---------------------------------------------------------------- a prompt, in chains
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk", [128, 37])
+def test_prompt_in_chains(chunk):
+    """Prompts of 300 and 170 ids (and none) go into a DraftCache as chains of up to ``chunk`` nodes, every one attended to and kept
+    whole; a sequence that has no more is absent.  The rows are those of causal attention over the whole prompt."""
+    lens, L, H, Hkv, D = [300, 170, 0], 2, 4, 2, 64
+    B, g = len(lens), torch.Generator().manual_seed(91)
+    r = lambda h: torch.randn(L, B, max(lens), h, D, generator=g).to(BF)  # noqa: E731
+    q, k, v = r(H), r(Hkv), r(Hkv)
+    cache = draft.DraftCache(L, B, 320, Hkv, D, BF, page_size=16)
+    got = torch.zeros(L, B, max(lens), H, D, dtype=BF)
+    for at in range(0, max(lens), chunk):
+        here = [max(0, min(n - at, chunk)) for n in lens]
+        N = max(here)
+        parents = torch.arange(-1, N - 1, dtype=torch.int32).repeat(B, 1)
+        for b, n in enumerate(here):
+            if n < N:
+                parents[b, n] = -2  # (what hangs on it is absent too: the rest, or all of a sequence without a root)
+        kk, vv = k[:, :, at:at + N].cuda(), v[:, :, at:at + N].cuda()
+        for l in range(L):
+            got[l, :, at:at + N] = cache.attend(l, q[l, :, at:at + N].cuda(), kk[l], vv[l], parents.cuda()).cpu()
+        path = torch.arange(N, dtype=torch.int32, device="cuda").repeat(B, 1)
+        cache.keep(kk, vv, draft.Verified(torch.tensor(here, dtype=torch.int32).cuda(), path, None))
+    assert cache.lens.tolist() == lens
+    eps = torch.finfo(BF).eps
+    for l in range(L):
+        for b, n in enumerate(lens):
+            assert not got[l, b, n:].any()
+            for h in range(H):
+                kd, vd = (x[l, b, :n, h // (H // Hkv)].double() for x in (k, v))
+                s = (q[l, b, :n, h].double() @ kd.t() * D ** -0.5).masked_fill(~torch.ones(n, n).tril().bool(), -torch.inf)
+                w = torch.softmax(s, -1)
+                want, mag = w @ vd, w @ vd.abs()
+                assert ((got[l, b, :n, h].double() - want).abs() <= (eps + 2.0 ** -8) * mag + eps / 2 * want.abs() + 2.0 ** -24).all()
