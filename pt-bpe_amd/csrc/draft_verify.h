@@ -19,12 +19,11 @@
 //
 // What has to be read: an entry of p and q for every node, and the rows of the contexts that a sum is needed of: the
 // last one's for the next id, others' only between a rejected child and its next sibling, and with ranges once for P and Q
-// of those with drafted children.  r is worked out anew from the
-// rows and the Z so far whenever it is needed, never stored.  One workgroup does a sequence: a row of 128 k entries takes
-// it about as long as the rows' share of the card's bandwidth once there are 100 sequences: 128 chains of 7 drafts over
-// 131072 fp32 entries take 33 us, 134 MB at 4.0 TB/s.  Small calls are dependent loads: one chain over 1091 ids 5.3 us, 48
-// trees of 40 nodes over 5123 ids held to ranges 18.5 (the longest walk: a sum for every context with children, and one per
-// rejected sibling).
+// of those with drafted children.  r is worked out anew from the rows and the Z so far whenever it is needed, never stored.
+// One workgroup does a sequence: a row of 128 k entries takes it about as long as the rows' share of the card's bandwidth
+// once there are 100 sequences: 128 chains of 7 drafts over 131072 fp32 entries take 33 us, 134 MB at 4.0 TB/s.  Small
+// calls are dependent loads: one chain over 1091 ids 5.3 us, 48 trees of 40 nodes over 5123 ids held to ranges 18.6 (the
+// longest walk: a sum for every context with children, and one per rejected sibling).
 #pragma once
 
 #include "draft.h"
