@@ -8,9 +8,13 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstdlib>
+#include <functional>
 #include <initializer_list>
 #include <string>
+#include <utility>
 
 #include "../../include/geobpe.h"
 
@@ -102,6 +106,37 @@ bool meet(const at::Tensor& x, const at::Tensor& y) {
   }
   return from[0] < to[1] && from[1] < to[0];
 }
+
+// Whether elements of two tensors of x's sizes and strides, the second `apart` elements further on, share memory (of one tensor,
+// apart = 0: two different elements): index differences d with sum d stride = apart.  Largest strides first: of an ordinary
+// layout's only a d or two a dimension leave what the smaller ones can make up for.
+struct Shared {
+  static constexpr int MOST = 5;             // dimensions of a cache
+  std::pair<int64_t, int64_t> dims[MOST];    // stride, size
+  int64_t rest[MOST + 1] = {}, steps = 0;    // what the dimensions from i on span at most
+  int n_dims = 0;
+  bool nested = true;  // every stride passes over what the smaller ones span: no two elements of the tensor meet
+  explicit Shared(const at::Tensor& x) {
+    for (int64_t i = 0; i < x.dim(); i++)
+      if (x.size(i) > 1) dims[n_dims++] = {x.stride(i), x.size(i)};
+    std::sort(dims, dims + n_dims, std::greater<>());
+    for (int i = n_dims; i-- > 0;) {
+      rest[i] = rest[i + 1] + dims[i].first * (dims[i].second - 1);
+      nested = nested && dims[i].first > rest[i + 1];
+    }
+  }
+  bool any(int64_t apart, int i, bool differ) {
+    if (i == n_dims) return apart == 0 && differ;
+    if (std::abs(apart) > rest[i] || ++steps > 10000) return false;  // (strides of no ordinary layout: not looked through)
+    const int64_t s = dims[i].first, n = dims[i].second;
+    if (s == 0) return any(apart, i + 1, true);  // (the smallest: all others were chosen)
+    int64_t from = (apart - rest[i + 1]) / s - 1, to = (apart + rest[i + 1]) / s + 1;
+    from = std::max(from, 1 - n), to = std::min(to, n - 1);
+    for (int64_t d = from; d <= to; d++)
+      if (any(apart - d * s, i + 1, differ || d)) return true;
+    return false;
+  }
+};
 
 bool unit(const at::Tensor& x) { return x.size(-1) <= 1 || x.stride(-1) == 1; }
 
@@ -326,13 +361,17 @@ PyObject* commit(PyObject*, PyObject* const* o, Py_ssize_t nargs) {
   for (int i = 0; i < 4; i++) {
     st[i][0] = 0;
     rows(names[i], *all[i], st[i] + !layers, 1);
-    for (int64_t d = 0; i > 1 && d < all[i]->dim(); d++)
-      if (all[i]->stride(d) == 0 && all[i]->size(d) > 1) VALUE("%s is expanded: its rows share memory", names[i]);
+    if (i < 2) continue;
+    Shared own(*all[i]);
+    if (!own.nested && own.any(0, 0, false)) VALUE("%s is expanded or its rows overlap: they share memory", names[i]);
   }
   for (int i = 0; i < 2; i++)
     if (meet(*x[i], *c.k) || meet(*x[i], *c.v))
       VALUE("%s lies in the cache's own memory, which the call writes: pass %s.clone()", names[i], names[i]);
   if (c.k->data_ptr() == c.v->data_ptr()) VALUE("v_cache is k_cache: each needs memory of its own");
+  if (c.k->strides() == c.v->strides() && meet(*c.k, *c.v) &&
+      Shared(*c.k).any(((const char*)c.v->data_ptr() - (const char*)c.k->data_ptr()) / e, 0, true))
+    VALUE("v_cache is partly k_cache: each needs memory of its own");
   const hipStream_t stream = stream_of(dev);
   at::Tensor out = at::empty({c.B}, c.lens->options());
   a.d_k = x[0]->data_ptr(), a.d_v = x[1]->data_ptr(), a.d_k_cache = c.k->data_ptr(), a.d_v_cache = c.v->data_ptr();

@@ -108,7 +108,7 @@ def commit(k_cache, v_cache, block_table, lens, k, v, path, n):
     any type whose rows are multiples of 16 bytes; path (B, N) and n (B,) as ``verify`` returns them.  The table has
     to have the pages for the new positions.  A kept node outside the tree, the table or the cache is not written,
     and that sequence's new length is -1.  Pages that sequences share must not be among the written ones, k and v not lie
-    in the cache's own memory, and a cache for both keys and values is refused."""
+    in the cache's own memory; a cache for both keys and values, or one whose rows overlap, is refused."""
     return (_bound or _ops()).commit(k_cache, v_cache, block_table, lens, k, v, path, n)
 
 

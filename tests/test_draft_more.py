@@ -432,6 +432,66 @@ def test_attention_rows_without_weights(N, lens):
     check_attention(attend(on(c)), want, BF)
 
 
+# ---------------------------------------------------------------- caches that share memory
+def caches_of_one(kind, L, P, S, H, D, dtype=BF, device="cpu"):
+    """Keys' and values' cache in one tensor, without an element in common."""
+    z = lambda *s: torch.zeros(*s, dtype=dtype, device=device)  # noqa: E731
+    if kind == "pages":
+        both = z(L, P, 2, S, H, D)
+        return both[:, :, 0], both[:, :, 1]
+    if kind == "heads":
+        both = z(L, P, S, H, 2 * D)
+        return both[..., :D], both[..., D:]
+    if kind == "layers":
+        both = z(2, L, P, S, H, D)
+        return both[0], both[1]
+    if kind == "heads first":
+        both = z(L, P, 2, H, S, D).transpose(3, 4)
+        return both[:, :, 0], both[:, :, 1]
+    both = z(L, 2 * P, S, H, D)
+    return both[:, 1::2], both[:, 0::2]
+
+
+KINDS = ["pages", "heads", "layers", "heads first", "turns"]
+
+
+def test_commit_refuses_caches_that_overlap():
+    """One a few pages, slots or heads further on in the other's memory, rows that overlap in a cache: two writes to one
+    place.  Caches that only lie in one tensor are none of these."""
+    c = make_commit(0, 2, 3, 4, [0, 5, 7], 2, 16, 4, BF)
+    L, P, S, H, D = c["k_cache"].shape
+    for kind in KINDS:
+        k, v = caches_of_one(kind, L, P, S, H, D)
+        refuse(commit, c, ValueError, "HIP device only", k_cache=k, v_cache=v)
+        refuse(commit, c, ValueError, "HIP device only", k_cache=v, v_cache=k)
+    pages, slots, heads = (torch.zeros(L, P + a, S + b, H + h, D, dtype=BF) for a, b, h in ((1, 0, 0), (0, 1, 0), (0, 0, 1)))
+    refuse(commit, c, ValueError, "partly k_cache", k_cache=pages[:, 1:], v_cache=pages[:, :-1])
+    refuse(commit, c, ValueError, "partly k_cache", k_cache=pages[:, :-1], v_cache=pages[:, 1:])
+    refuse(commit, c, ValueError, "partly k_cache", k_cache=slots[:, :, 1:], v_cache=slots[:, :, :-1])
+    refuse(commit, c, ValueError, "partly k_cache", k_cache=heads[:, :, :, :-1], v_cache=heads[:, :, :, 1:])
+    wide = torch.zeros(L, P, S, H, 2 * D, dtype=BF)
+    refuse(commit, c, ValueError, "partly k_cache", k_cache=wide[..., :D], v_cache=wide[..., 8:D + 8])
+    flat = torch.zeros(L * P * S * H * D, dtype=BF)
+    near = torch.as_strided(flat, (L, P, S, H, D), (P * S * H * D, S * H * D, H * D, 8, 1))  # heads half a head apart
+    refuse(commit, c, ValueError, "overlap", k_cache=near)
+    refuse(commit, c, ValueError, "overlap", v_cache=torch.as_strided(flat, (L, P, S, H, D), (P * 8, 8, H * D, D, 1)))
+    refuse(commit, c, ValueError, "expanded", v_cache=c["v_cache"][:, :, :1].expand(-1, -1, S, -1, -1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_commit_into_caches_of_one_tensor(kind):
+    from test_draft import ref_commit
+    c = make_commit(76, 3, 4, 6, [0, 15, 16, 17], 2, 48, 16, BF)
+    kc, vc, want = ref_commit(c)
+    d = on(c)
+    k, v = caches_of_one(kind, *c["k_cache"].shape, device="cuda")
+    k.copy_(d["k_cache"])
+    v.copy_(d["v_cache"])
+    assert torch.equal(commit({**d, "k_cache": k, "v_cache": v}).cpu(), want)
+    assert torch.equal(k.cpu(), kc) and torch.equal(v.cpu(), vc)
+
+
 @pytest.mark.gpu
 def test_commit_tells_autograd_of_its_writes():
     """A cache that a later backward pass needs as it was: torch has to see that it was written."""
