@@ -1,5 +1,6 @@
 """More of the decoding operators (geobpe.draft) against plain 64-bit implementations: rows held to id ranges that have
-mass outside them, scales and scores at the ends of float32, long contexts with every tile visible, what autograd is told.
+mass outside them, scales and scores at the ends of float32, long contexts with every tile visible, a prompt in chains, caches
+that share memory, what autograd is told.
 
 Attention's tolerance is test_draft.py's, from the same count of roundings."""
 import ctypes
@@ -14,7 +15,7 @@ import torch
 from conftest import REPO
 from geobpe import draft
 from test_draft import (_ATTEND, _Vocabulary, attend, check_attention, check_verify, commit, make_attention, make_commit,
-                        make_parents, make_verify, on, ref_attention, ref_verify, refuse, tree_paths, verify)
+                        make_verify, on, ref_attention, ref_verify, refuse, tree_paths, verify)
 
 BF, FP = torch.bfloat16, torch.float16
 
